@@ -65,6 +65,11 @@ def _declare(lib: ctypes.CDLL) -> None:
         "gfs_rmsnorm_bwd_parts": ([i], i),
         "gfs_rmsnorm_bwd": ([vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, vp], i),
         "gfs_rope": ([vp, vp, vp, i, i, i, i, i, cl, i, i, vp], i),
+        "gfs_rotary": ([vp, vp, lp, vp, vp, vp, i, i, i, i, i, i, i, i, i, i, vp], i),
+        "gfs_qk_norm_rope_fwd": ([vp, lp, vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, i, i, f, i, vp], i),
+        "gfs_qk_norm_rope_scratch": ([i], i64),
+        "gfs_qk_norm_rope_bwd": ([vp, vp, vp, vp, vp, lp, vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, i, i, f, i,
+                                  vp], i),
         "gfs_swiglu_fwd": ([vp, vp, i, i, vp], i),
         "gfs_swiglu_bwd": ([vp, vp, vp, i, i, vp], i),
         "gfs_embedding_fwd": ([vp, vp, vp, i, i, i, i, i, i, i, vp], i),
@@ -184,6 +189,11 @@ def stream_ptr() -> int:
     """Raw handle of the current stream (``torch.cuda.current_stream()`` builds a Stream object: 4 us per
     launch, this 0.2 us)."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def on_device(t: torch.Tensor):
+    """``with on_device(t):`` launches on ``t``'s device and its current stream (free where that is the current device)."""
+    return _NULL_RANGE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def ptr(t: torch.Tensor | None) -> int:
