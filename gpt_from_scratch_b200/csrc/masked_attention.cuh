@@ -1,0 +1,68 @@
+// The mask and the scores of masked attention (masked_attention.cu, masked_attention_bwd.cu).
+//
+// Every query sees one range of keys, [first, last), and both ends grow or stay from query to query of a sequence:
+// documents, a prefix, a window and padding all have that form. So the queries that see a key are a range too, the ends of a tile's
+// first and last row bound the whole tile, and a block of scores is skipped, masked or taken whole by comparing numbers.
+#pragma once
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace gfs {
+
+// What gfs_attention_mask writes; int32, S_pad = S rounded up to a multiple of 128. A token whose two ranges are empty is
+// padding: it sees nothing and nothing sees it, and what its rows of q, k, v and the gradients hold does not matter.
+// Rows S .. S_pad are empty.
+struct MaskView {
+  const int *first, *last;     // [B, S_pad]: the keys that a query sees
+  const int *qfirst, *qlast;   // [B, S_pad]: the queries that see a key
+  const int* padded;           // [B]: the sequence has padding
+};
+
+// The softmax's exponents are base 2: score = log2(e) (scale q k, or cap tanh(scale q k / cap)) - slope log2(e) |i - j|.
+struct ScoreArgs {
+  float sl2;            // scale log2(e); capped: 2 scale log2(e) / cap, so that tanh(..) = 1 - 2 / (1 + 2^(sl2 q k))
+  float cap2;           // cap log2(e)
+  const float* slopes;  // [heads], or null
+};
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// r = 1 / (1 + 2^(sl2 x)) of four scores: tanh = 1 - 2 r, its derivative 4 r (1 - r). The absolute error counts here
+// (the score is an exponent), and it is that of r, a few 2^-24: the approximate tanh instruction is off by up to 2^-11 of the
+// value, 0.02 for a score of 40. Four exponentials and one reciprocal, of the product of the four denominators: it stays in range as
+// exponents are cut off at 30, where tanh is 1 to 32 bits.
+__device__ __forceinline__ void sigmoids(const float (&x)[4], float sl2, float (&r)[4]) {
+  float d[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d[i] = 1.f + fast_exp2(min_nan(x[i] * sl2, 30.f));
+  const float a = d[0] * d[1], b = d[2] * d[3], inv = fast_rcp(a * b);
+  const float ra = inv * b, rb = inv * a;
+  r[0] = ra * d[1];
+  r[1] = ra * d[0];
+  r[2] = rb * d[3];
+  r[3] = rb * d[2];
+}
+
+// Zeros in the rows of a tile (swizzled blocks of 64 columns, `rows` rows of 128 bytes, `blocks` of them block_bytes apart) whose
+// tokens are padding: their probabilities are 0, but 0 times what they hold might not be. The whole warp.
+__device__ __forceinline__ void zero_padding(uint8_t* tile, int rows, int blocks, int block_bytes, const int* first,
+                                             const int* last, int lane) {
+  for (int r0 = 0; r0 < rows; r0 += 32) {
+    unsigned dead = __ballot_sync(0xffffffffu, first[r0 + lane] >= last[r0 + lane]);
+    while (dead != 0u) {
+      const int r = r0 + __ffs(dead) - 1;
+      dead &= dead - 1;
+      for (int c = lane; c < blocks * 8; c += 32)
+        *reinterpret_cast<uint4*>(tile + (c >> 3) * block_bytes + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+}  // namespace gfs

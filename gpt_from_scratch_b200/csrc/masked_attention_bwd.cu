@@ -1,0 +1,590 @@
+// Masked attention, backward (head_dim 64 or 128, bf16; the mask and the scores: masked_attention.cuh).
+//
+//   P = 2^(score - lse), dP = dO V^T, dvec = rowsum(dO * O), dS = P (dP - dvec) (times 1 - tanh^2 of capped scores)
+//   dV = P^T dO, dK = scale dS^T Q (both summed over the heads of q that share them), dQ = scale dS K
+//
+// Two kernels from one template, deterministic, no atomics, after a pre-pass for dvec:
+//   mode 0: items of 128 keys    -> dK, dV, streaming 64-query tiles of every head of the group
+//   mode 1: items of 128 queries -> dQ,     streaming 64-key tiles
+// Only the streamed tiles between the item's first and last visible row are visited. Both modes recompute P from two score MMAs
+// (X = R1 T1^T, Y = R2 T2^T) and hand P / dS (bf16) to the gradient MMAs through tensor memory; the streamed tile is
+// consumed twice from the same shared-memory bytes, K-major and MN-major.
+#include <algorithm>
+
+#include "api.h"
+#include "attention_tiles.cuh"
+#include "masked_attention.cuh"
+
+using namespace gfs;
+using gfs_host::make_map;
+using gfs_host::strides_ok;
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// Pre-pass: dvec[b, h, s] = sum_d dO * O, 0 for padding (whatever its dO holds) and for rows S .. S_pad. D / 8 threads
+// per row, 16-byte loads, rows in the memory order of O (heads or tokens fastest).
+// ---------------------------------------------------------------------------
+constexpr int DVEC_ROWS = 4;
+__global__ void __launch_bounds__(256)
+masked_dvec_kernel(const __nv_bfloat16* dO, const __nv_bfloat16* O, float* __restrict__ dvec, const int* first,
+                   const int* last, int S, int S_pad, int B, int nh, int D, long long do_ss, long long do_bs,
+                   long long do_hs, long long o_ss, long long o_bs, long long o_hs, int s_fastest) {
+  pdl_wait();
+  pdl_trigger();
+  const int tpr = D >> 3;                       // 8 or 16 threads per row
+  const int rows_per_pass = blockDim.x / tpr;
+  const int sub = threadIdx.x % tpr;
+  const unsigned total = static_cast<unsigned>(S_pad) * B * nh;
+  const unsigned row0 = blockIdx.x * static_cast<unsigned>(rows_per_pass * DVEC_ROWS) + threadIdx.x / tpr;
+  uint4 x[DVEC_ROWS], y[DVEC_ROWS];
+  unsigned at[DVEC_ROWS];
+#pragma unroll
+  for (int i = 0; i < DVEC_ROWS; ++i) {
+    const unsigned row = row0 + i * rows_per_pass;
+    x[i] = y[i] = make_uint4(0, 0, 0, 0);
+    unsigned h, b, s;
+    if (s_fastest) {
+      s = row % S_pad;
+      const unsigned bh = row / S_pad;
+      h = bh % nh;
+      b = bh / nh;
+    } else {
+      h = row % nh;
+      const unsigned sb = row / nh;
+      b = sb % B;
+      s = sb / B;
+    }
+    at[i] = (b * nh + h) * S_pad + s;
+    if (row < total && s < static_cast<unsigned>(S) && first[b * S_pad + s] < last[b * S_pad + s]) {
+      x[i] = *reinterpret_cast<const uint4*>(dO + s * do_ss + b * do_bs + h * do_hs + sub * 8);
+      y[i] = *reinterpret_cast<const uint4*>(O + s * o_ss + b * o_bs + h * o_hs + sub * 8);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < DVEC_ROWS; ++i) {
+    const unsigned row = row0 + i * rows_per_pass;
+    const uint32_t xw[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    const uint32_t yw[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+    float acc = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 a2 = unpack_bf16x2(xw[e]), b2 = unpack_bf16x2(yw[e]);
+      acc += a2.x * b2.x + a2.y * b2.y;
+    }
+    for (int o = tpr >> 1; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    if (row < total && sub == 0) dvec[at[i]] = acc;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Main kernel
+// ---------------------------------------------------------------------------
+struct MaskedBwdParams {
+  __nv_bfloat16* out1;  // mode 0: dK, mode 1: dQ
+  __nv_bfloat16* out2;  // mode 0: dV
+  long long o1_ss, o1_bs, o1_hs;
+  long long o2_ss, o2_bs, o2_hs;
+  const float* lse;   // [B, nh, S_pad], base 2
+  const float* dvec;  // [B, nh, S_pad]
+  int S, S_pad, B, nh, group;
+  float scale;
+  ScoreArgs score;
+  MaskView mask;
+  uint32_t* status;
+};
+
+constexpr int MBWD_CW = 16;                         // compute warps
+constexpr int MBWD_FIRST_CW = 4;                    // warps 0-2: TMA, score MMAs, gradient MMAs; 3: idle
+constexpr int MBWD_THREADS = 32 * (MBWD_FIRST_CW + MBWD_CW);
+
+template <int D, int MODE>
+struct MBwdShape {
+  // Stages of the streamed-tile ring. A stage is only released when the gradient MMAs that read it have
+  // finished and the score MMAs run two tiles ahead, so the TMA of a tile has (TS - 2) tile periods to land.
+  static constexpr int TS = D == 64 ? 7 : 4;
+  static constexpr int STAGE_BYTES = 2048;          // per compute warp, to transpose its output rows through
+  static constexpr int STAGING = MBWD_CW * STAGE_BYTES;
+  static constexpr int SMEM = 2 * (D / 64) * 16384 + 2 * TS * (D / 64) * 8192 + STAGING + (MODE == 0 ? TS * 512 : 0) + 256;
+};
+
+// Sixteen compute warps: two groups of eight take alternate streamed tiles (group = X/Y buffer); within a group two warps
+// share the 32 rows of a quarter, 32 streamed columns each (no exchange is needed: the statistics are inputs). The
+// MMAs are issued by two warps (1: scores, 2: gradients), so neither order waits for the other. P / dS go to columns of their own
+// where there is room, for dK / dV at head_dim 128 to the columns of the scores they were made from.
+template <int D, int MODE, bool CAP, bool DIST>
+__global__ void __launch_bounds__(MBWD_THREADS, 1)
+masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant__ CUtensorMap tr2,
+                  const __grid_constant__ CUtensorMap tt1, const __grid_constant__ CUtensorMap tt2,
+                  const MaskedBwdParams p, int n_rt, int n_items) {
+  using Shape = MBwdShape<D, MODE>;
+  constexpr int DB = D / 64;
+  constexpr int TS = Shape::TS;
+  constexpr int R_BYTES = DB * 16384;  // resident [128 x D]
+  constexpr int T_BYTES = DB * 8192;   // streamed [64 x D]
+  constexpr uint32_t TMEM_COLS = 512;
+  constexpr uint32_t Y_COL = 128;      // X tiles at [0, 128), Y tiles after them
+  constexpr uint32_t ACC1 = 256, ACC2 = 256 + D;
+  constexpr bool OVERLAY = (D == 128 && MODE == 0);   // P over X, dS over Y
+  constexpr uint32_t PT_COL = 384;     // else: [buffer][P 32 cols | dS 32 cols]
+  constexpr int EPI_WARPS = (MODE == 1 && D == 64) ? MBWD_CW / 2 : MBWD_CW;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* R1 = smem_raw;
+  uint8_t* R2 = R1 + R_BYTES;
+  uint8_t* T1 = R2 + R_BYTES;
+  uint8_t* T2 = T1 + TS * T_BYTES;
+  uint8_t* staging = T2 + TS * T_BYTES;
+  float* stats = reinterpret_cast<float*>(staging + Shape::STAGING);  // mode 0: [TS stages][lse 64 | dvec 64]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(stats) + (MODE == 0 ? TS * 512 : 0));
+  uint64_t* r_full = bars;
+  uint64_t* t_full = bars + 1;             // [TS]
+  uint64_t* t_empty = t_full + TS;         // [TS]
+  uint64_t* xy_full = t_empty + TS;
+  uint64_t* xy_empty = xy_full + 2;
+  uint64_t* m_full = xy_empty + 2;
+  uint64_t* m_empty = m_full + 2;
+  uint64_t* acc_full = m_empty + 2;
+  uint64_t* acc_empty = acc_full + 1;
+  uint64_t* r_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 3);
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (smem_u32(smem_raw) & 1023u) {
+    if (threadIdx.x == 0) record_status(p.status, STATUS_BAD_ARGUMENT, 0x5a23u);
+    return;
+  }
+  const int heads = MODE == 0 ? p.nh / p.group : p.nh;
+  const int BH = p.B * heads;
+  // the rows that a resident row sees: queries of a key, keys of a query
+  const int* const lo_all = MODE == 0 ? p.mask.qfirst : p.mask.first;
+  const int* const hi_all = MODE == 0 ? p.mask.qlast : p.mask.last;
+  // Persistent: a CTA walks work items (resident tile, batch * head) dealt in a snake over the CTAs; barrier phases
+  // run on counters that continue across items, so the next item's loads and first score MMAs overlap this one's epilogue.
+  const int G = static_cast<int>(gridDim.x);
+  auto snake = [&](int rnd) {
+    return rnd * G + ((rnd & 1) ? G - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
+  };
+  // resident tile, batch and head of work item w, its first streamed tile and their number per head (at least one, which
+  // may be masked whole)
+  auto decode = [&](int w, int& rt, int& b, int& h, int& t_begin, int& n_t) {
+    const int level = w / BH;
+    const int bh = w % BH;
+    rt = MODE == 0 ? level : n_rt - 1 - level;   // under a causal mask the heaviest come first
+    b = bh / heads;
+    h = bh % heads;
+    const size_t row = static_cast<size_t>(b) * p.S_pad;
+    t_begin = lo_all[row + rt * 128] >> 6;
+    n_t = max(((hi_all[row + min(rt * 128 + 127, p.S - 1)] + 63) >> 6) - t_begin, 1);
+  };
+
+  if (threadIdx.x == 0) {
+    mbar_init(r_full, 1);
+    for (int i = 0; i < TS; ++i) {
+      mbar_init(&t_full[i], 1);
+      mbar_init(&t_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&xy_full[i], 1);
+      mbar_init(&xy_empty[i], MBWD_CW / 2);
+      mbar_init(&m_full[i], MBWD_CW / 2);
+      mbar_init(&m_empty[i], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, EPI_WARPS);
+    mbar_init(r_empty, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tr1);
+    tma_prefetch_desc(&tr2);
+    tma_prefetch_desc(&tt1);
+    tma_prefetch_desc(&tt2);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // Set-up above may overlap the tail of the preceding kernel (programmatic launch). The dQ kernel reads nothing that the
+  // preceding dK / dV kernel writes, and that one had waited for everything before it when it let this one start: it
+  // waits at its end, so that its completion means that of both (launch_hints.h).
+  if (MODE == 0) pdl_wait();
+  pdl_trigger();
+  const uint32_t tmem_base = *tmem_slot;
+  WaitCtx wctx{abort_flag, p.status, GFS_WAIT_LIMIT_NS};
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int g = 0;  // streamed tiles loaded so far (ring position)
+      for (int it = 0; it * G < n_items; ++it) {
+        const int w = snake(it);
+        if (w >= n_items) break;
+        int rt, b, h, t_begin, n_t;
+        decode(w, rt, b, h, t_begin, n_t);
+        mbar_wait(r_empty, (it & 1) ^ 1u, wctx, STATUS_TIMEOUT_PIPE_EMPTY);  // previous item's score MMAs done
+        mbar_arrive_expect_tx(r_full, 2 * R_BYTES);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          tma_load_4d(R1 + db * 16384, &tr1, r_full, db * 64, rt * 128, h, b);
+          tma_load_4d(R2 + db * 16384, &tr2, r_full, db * 64, rt * 128, h, b);
+        }
+        const int n_heads = MODE == 0 ? p.group : 1;
+        for (int hh = 0; hh < n_heads; ++hh) {
+          const int th = MODE == 0 ? h * p.group + hh : h / p.group;   // head of the streamed tiles
+          for (int t = 0; t < n_t; ++t, ++g) {
+            const int st = g % TS;
+            const int ti = t_begin + t;
+            mbar_wait(&t_empty[st], ((g / TS) & 1) ^ 1u, wctx, STATUS_TIMEOUT_PIPE_EMPTY);
+            mbar_arrive_expect_tx(&t_full[st], 2 * T_BYTES + (MODE == 0 ? 512 : 0));
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+              tma_load_4d(T1 + st * T_BYTES + db * 8192, &tt1, &t_full[st], db * 64, ti * 64, th, b);
+              tma_load_4d(T2 + st * T_BYTES + db * 8192, &tt2, &t_full[st], db * 64, ti * 64, th, b);
+            }
+            if (MODE == 0) {
+              const size_t off = (static_cast<size_t>(b) * p.nh + th) * p.S_pad + ti * 64;
+              bulk_load_1d(stats + st * 128, p.lse + off, 256, &t_full[st]);
+              bulk_load_1d(stats + st * 128 + 64, p.dvec + off, 256, &t_full[st]);
+            }
+          }
+        }
+      }
+      settle_copies(wctx);
+    }
+  } else if (warp == 1) {
+    // Score MMAs (whole warp, converged: the MMA / commit helpers elect the issuing lane); runs ahead as
+    // far as the X/Y buffers and the streamed-tile ring allow.
+    constexpr uint32_t idesc_xy = umma_idesc_bf16(128, 64, 0, 0);
+    const uint32_t r1 = smem_u32(R1), r2 = smem_u32(R2);
+    int g = 0;
+    for (int it = 0; it * G < n_items; ++it) {
+      const int w = snake(it);
+      if (w >= n_items) break;
+      int rt, b, h, t_begin, n_t;
+      decode(w, rt, b, h, t_begin, n_t);
+      const bool padded = p.mask.padded[b] != 0;
+      const int n = MODE == 0 ? n_t * p.group : n_t;
+      mbar_wait(r_full, it & 1, wctx, STATUS_TIMEOUT_PIPE_FULL);
+      for (int t = 0; t < n; ++t, ++g) {
+        const int st = g % TS, sb = g & 1;
+        mbar_wait(&t_full[st], (g / TS) & 1, wctx, STATUS_TIMEOUT_PIPE_FULL);
+        if (padded) {
+          const size_t at = static_cast<size_t>(b) * p.S_pad + (t_begin + t % n_t) * 64;
+          zero_padding(T1 + st * T_BYTES, 64, DB, 8192, p.mask.first + at, p.mask.last + at, lane);
+          zero_padding(T2 + st * T_BYTES, 64, DB, 8192, p.mask.first + at, p.mask.last + at, lane);
+        }
+        mbar_wait(OVERLAY ? &m_empty[sb] : &xy_empty[sb], ((g >> 1) & 1) ^ 1u, wctx, STATUS_TIMEOUT_SOFTMAX);
+        tc_fence_after();
+        mma_kk<D / 16>(tmem_base + sb * 64, r1, 16384, smem_u32(T1 + st * T_BYTES), 8192, idesc_xy, false);
+        mma_kk<D / 16>(tmem_base + Y_COL + sb * 64, r2, 16384, smem_u32(T2 + st * T_BYTES), 8192, idesc_xy, false);
+        umma_commit_e(&xy_full[sb]);
+      }
+      umma_commit_e(r_empty);
+    }
+  } else if (warp == 2) {
+    // gradient MMAs
+    constexpr uint32_t idesc_acc = umma_idesc_bf16(128, D, 0, 1);
+    int g = 0;
+    for (int it = 0; it * G < n_items; ++it) {
+      const int w = snake(it);
+      if (w >= n_items) break;
+      int rt, b, h, t_begin, n_t;
+      decode(w, rt, b, h, t_begin, n_t);
+      const int n = MODE == 0 ? n_t * p.group : n_t;
+      for (int t = 0; t < n; ++t, ++g) {
+        const int st = g % TS, sb = g & 1;
+        mbar_wait(&m_full[sb], (g >> 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
+        if (t == 0) mbar_wait(acc_empty, (it & 1) ^ 1u, wctx, STATUS_TIMEOUT_TMEM_EMPTY);  // previous epilogue done
+        tc_fence_after();
+        const uint32_t pt = tmem_base + (OVERLAY ? sb * 64 : PT_COL + sb * 64);
+        const uint32_t ds = OVERLAY ? pt + Y_COL : pt + 32;
+        constexpr int HALF = OVERLAY ? 32 : 16;   // columns from the first to the second half of P / dS
+        if (MODE == 0) {
+          mma_tmn<4, HALF>(tmem_base + ACC1, pt, smem_u32(T2 + st * T_BYTES), 8192, idesc_acc, t > 0);   // dV += P^T dO
+          mma_tmn<4, HALF>(tmem_base + ACC2, ds, smem_u32(T1 + st * T_BYTES), 8192, idesc_acc, t > 0);   // dK += dS^T Q
+        } else {
+          mma_tmn<4, HALF>(tmem_base + ACC1, ds, smem_u32(T1 + st * T_BYTES), 8192, idesc_acc, t > 0);   // dQ += dS K
+        }
+        umma_commit_e(&t_empty[st]);
+        umma_commit_e(&m_empty[sb]);
+      }
+      umma_commit_e(acc_full);
+    }
+  } else if (warp >= MBWD_FIRST_CW) {
+    const int cw = warp - MBWD_FIRST_CW;
+    const int quarter = warp & 3;
+    const int half = (cw >> 2) & 1;     // 32 of the 64 streamed columns
+    const int group = cw >> 3;          // parity of the streamed tiles of this warp
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const float sl2 = p.score.sl2, cap2 = p.score.cap2;
+    const uint64_t neg_sl2 = pack_f32x2(-sl2, -sl2), neg_one = pack_f32x2(-1.f, -1.f);
+    const uint32_t x_addr = tmem_base + lane_base + group * 64 + half * 32;
+    const uint32_t y_addr = x_addr + Y_COL;
+    const uint32_t p_addr = OVERLAY ? x_addr : tmem_base + lane_base + PT_COL + group * 64 + half * 16;
+    const uint32_t ds_addr = OVERLAY ? y_addr : p_addr + 32;
+    uint8_t* stage = staging + cw * Shape::STAGE_BYTES;
+    bool acc_pending = false;           // the previous item's acc_full phase has not been waited for
+    int g0 = 0;
+    for (int it = 0; it * G < n_items; ++it) {
+      const int w = snake(it);
+      if (w >= n_items) break;
+      int rt, b, h, t_begin, n_t;
+      decode(w, rt, b, h, t_begin, n_t);
+      const int n = MODE == 0 ? n_t * p.group : n_t;
+      const int row_g = rt * 128 + r;  // mode 0: key position, mode 1: query position
+      const int* lo_b = lo_all + static_cast<size_t>(b) * p.S_pad;
+      const int* hi_b = hi_all + static_cast<size_t>(b) * p.S_pad;
+      const int lo = lo_b[row_g], hi = hi_b[row_g];
+      const int row0 = rt * 128 + quarter * 32, row_z = min(row0 + 31, p.S - 1);
+      // what every row of this warp sees, and what any of them does (a warp past the end: nothing)
+      const int lo_min = lo_b[row0], hi_min = hi_b[row0];
+      const int lo_max = row0 < p.S ? lo_b[row_z] : lo_min, hi_max = row0 < p.S ? hi_b[row_z] : hi_min;
+      float row_lse = 0.f, row_dvec = 0.f;
+      if (MODE == 1) {
+        row_lse = p.lse[(static_cast<size_t>(b) * p.nh + h) * p.S_pad + row_g];
+        row_dvec = p.dvec[(static_cast<size_t>(b) * p.nh + h) * p.S_pad + row_g];
+      }
+      for (int t = (g0 + group) & 1; t < n; t += 2) {
+        const int g = g0 + t;
+        const int st = g % TS;                      // streamed-tile stage (for the column statistics)
+        const uint32_t par = (g >> 1) & 1;
+        const int hh = MODE == 0 ? t / n_t : 0;
+        const int col0 = (t_begin + t - hh * n_t) * 64 + half * 32;       // position of this warp's first column
+        const int kind = col0 > hi_max - 1 || col0 + 31 < lo_min || hi_max <= lo_min ? 2      // nothing is seen
+                         : (col0 >= lo_max && col0 + 32 <= hi_min ? 0 : 1);                   // everything; some
+        mbar_wait(&xy_full[group], par, wctx, STATUS_TIMEOUT_SOFTMAX);
+        tc_fence_after();
+        uint32_t pp[16], dd[16];
+        if (kind == 2) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) pp[e] = dd[e] = 0u;
+          if (!OVERLAY && lane == 0) mbar_arrive(&xy_empty[group]);
+        } else {
+          uint32_t xv[32], yv[32];
+          tmem_ld_32x32(x_addr, xv);
+          tmem_ld_32x32(y_addr, yv);
+          tmem_ld_wait_for(xv);
+          tmem_ld_wait_for(yv);
+          if (!OVERLAY) {
+            // X / Y are in registers: hand the buffer back now so the next scores can be computed
+            // into it while this block's math runs
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&xy_empty[group]);
+          }
+          const float slope2 = DIST ? p.score.slopes[MODE == 0 ? h * p.group + hh : h] * LOG2E_F : 0.f;
+          const float dist0 = static_cast<float>(row_g - col0);
+          const int a = lo - col0;
+          const unsigned width = static_cast<unsigned>(hi - lo);
+          // Chunks seen in part turn their dead scores into -inf in the registers, which makes both P and dS exact
+          // zeros (dvec and dP are finite: padding was zeroed), and run the same code as the others.
+          if (!CAP && !DIST && kind == 1) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) xv[e] = static_cast<unsigned>(e - a) < width ? xv[e] : 0xff800000u;
+          }
+          const float* st_lse = stats + st * 128 + half * 32;
+          const float* st_dv = st_lse + 64;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            float ls[4], dv[4];
+            if (MODE == 0) {   // per-column statistics of the streamed query tile (same address in all lanes)
+              *reinterpret_cast<float4*>(ls) = *reinterpret_cast<const float4*>(st_lse + e);
+              *reinterpret_cast<float4*>(dv) = *reinterpret_cast<const float4*>(st_dv + e);
+            } else {
+              ls[0] = ls[1] = ls[2] = ls[3] = row_lse;
+              dv[0] = dv[1] = dv[2] = dv[3] = row_dvec;
+            }
+            float pr[4], slope[4];     // probabilities; derivative of the capped score / 4
+            if (CAP || DIST) {
+              float x[4], y[4];
+#pragma unroll
+              for (int u = 0; u < 4; ++u) x[u] = __uint_as_float(xv[e + u]);
+              if (CAP) {
+                float rr[4];
+                sigmoids(x, sl2, rr);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                  y[u] = fmaf(rr[u], -2.f * cap2, cap2);
+                  slope[u] = fmaf(-rr[u], rr[u], rr[u]);
+                }
+              } else {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) y[u] = x[u] * sl2;
+              }
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                if (DIST) y[u] = fmaf(fabsf(dist0 - static_cast<float>(e + u)), -slope2, y[u]);
+                if (kind == 1 && static_cast<unsigned>(e + u - a) >= width) y[u] = -INFINITY;
+                pr[u] = fast_exp2(y[u] - ls[u]);
+              }
+            } else {
+#pragma unroll
+              for (int u = 0; u < 4; u += 2) {
+                // 2^(x scale log2(e) - lse), two columns per instruction: formed negated, the exponential turns the sign back
+                const float2 z = unpack_f32x2(fma_f32x2(pack_u32x2(xv[e + u], xv[e + u + 1]), neg_sl2,
+                                                        pack_f32x2(ls[u], ls[u + 1])));
+                pr[u] = fast_exp2(-z.x);
+                pr[u + 1] = fast_exp2(-z.y);
+              }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u += 2) {
+              const uint64_t dy = fma_f32x2(pack_f32x2(dv[u], dv[u + 1]), neg_one, pack_u32x2(yv[e + u], yv[e + u + 1]));
+              uint64_t d2 = mul_f32x2(pack_f32x2(pr[u], pr[u + 1]), dy);
+              if (CAP) d2 = mul_f32x2(d2, pack_f32x2(4.f * slope[u], 4.f * slope[u + 1]));
+              const float2 d = unpack_f32x2(d2);
+              if (MODE == 0) pp[(e + u) >> 1] = pack_bf16x2(pr[u], pr[u + 1]);
+              dd[(e + u) >> 1] = pack_bf16x2(d.x, d.y);
+            }
+          }
+        }
+        // columns of this row -> 16 packed columns of the P / dS tensor-memory tiles
+        if (!OVERLAY) {
+          mbar_wait(&m_empty[group], par ^ 1u, wctx, STATUS_TIMEOUT_SOFTMAX);
+          tc_fence_after();
+        }
+        if (MODE == 0) tmem_st_32x16(p_addr, pp);
+        tmem_st_32x16(ds_addr, dd);
+        if (acc_pending) {   // before the arrival that lets the next phase of acc_full complete
+          mbar_wait(acc_full, (it - 1) & 1, wctx, STATUS_TIMEOUT_TMEM_FULL);
+          acc_pending = false;
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m_full[group]);
+      }
+      g0 += n;
+      // Epilogue: accumulators -> global. dK / dV: one group of warps each, a half of the columns per warp.
+      // dQ: a quarter of the columns per warp at head_dim 128; at head_dim 64 the group that does not own
+      // the next item's first tile does it all and the other one goes on.
+      if (EPI_WARPS != MBWD_CW && group == (g0 & 1)) {
+        acc_pending = true;
+        continue;
+      }
+      constexpr int NC = (MODE == 0) ? D / 64 : 1;    // 32-column chunks per warp
+      const int c0 = (MODE == 0) ? half * (D / 2) : (D == 128 ? group * 64 + half * 32 : half * 32);
+      const bool is_dv = MODE == 0 && group == 1;
+      const float out_scale = is_dv ? 1.f : p.scale;
+      const bool seen = lo < hi;                       // padding: zeros, whatever its own rows held
+      const long long o_ss = is_dv ? p.o2_ss : p.o1_ss;
+      __nv_bfloat16* out = is_dv ? p.out2 + row0 * p.o2_ss + b * p.o2_bs + h * p.o2_hs
+                                 : p.out1 + row0 * p.o1_ss + b * p.o1_bs + h * p.o1_hs;
+      const uint32_t acc = tmem_base + lane_base + (MODE == 0 && !is_dv ? ACC2 : ACC1);
+#pragma unroll
+      for (int ci = 0; ci < NC; ++ci) {
+        const int c = c0 + 32 * ci;
+        if (ci == 0) {
+          mbar_wait(acc_full, it & 1, wctx, STATUS_TIMEOUT_TMEM_FULL);
+          tc_fence_after();
+        }
+        uint32_t v[32], wv[16];
+        tmem_ld_32x32(acc + c, v);
+        tmem_ld_wait_for(v);
+        if (ci == NC - 1) {      // the accumulators may be overwritten by the next item
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          wv[e] = seen ? pack_bf16x2(__uint_as_float(v[2 * e]) * out_scale, __uint_as_float(v[2 * e + 1]) * out_scale) : 0u;
+        store_rows_32x32(stage, wv, lane, out + c, o_ss, p.S - row0);
+      }
+    }
+  }
+
+  if (MODE == 1) pdl_wait();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
+}
+
+struct BwdMaps {
+  const CUtensorMap *q128, *k128, *v128, *do128, *q64, *k64, *v64, *do64;
+};
+
+template <int D, bool CAP, bool DIST>
+int launch_bwd(const BwdMaps& m, const MaskedBwdParams& p0, const MaskedBwdParams& p1, cudaStream_t stream) {
+  static gfs_host::SmemLimit limit0, limit1;
+  const int n_rt = p0.S_pad / 128;
+  const int items0 = n_rt * p0.B * (p0.nh / p0.group), items1 = n_rt * p0.B * p0.nh;
+  constexpr int smem0 = MBwdShape<D, 0>::SMEM, smem1 = MBwdShape<D, 1>::SMEM;
+  if (!limit0.raise(masked_bwd_kernel<D, 0, CAP, DIST>, smem0) || !limit1.raise(masked_bwd_kernel<D, 1, CAP, DIST>, smem1))
+    return -10;
+  gfs_host::launch_pdl(masked_bwd_kernel<D, 0, CAP, DIST>, dim3(std::min(items0, gfs_host::sm_count())),
+                       dim3(MBWD_THREADS), smem0, stream, *m.k128, *m.v128, *m.q64, *m.do64, p0, n_rt, items0);
+  if (cudaGetLastError() != cudaSuccess) return -12;
+  gfs_host::launch_pdl(masked_bwd_kernel<D, 1, CAP, DIST>, dim3(std::min(items1, gfs_host::sm_count())),
+                       dim3(MBWD_THREADS), smem1, stream, *m.q128, *m.do128, *m.k64, *m.v64, p1, n_rt, items1);
+  return cudaGetLastError() == cudaSuccess ? 0 : -13;
+}
+template <int D>
+int launch_bwd_scores(const BwdMaps& m, const MaskedBwdParams& p0, const MaskedBwdParams& p1, bool cap, cudaStream_t s) {
+  const bool dist = p0.score.slopes != nullptr;
+  if (cap) return dist ? launch_bwd<D, true, true>(m, p0, p1, s) : launch_bwd<D, true, false>(m, p0, p1, s);
+  return dist ? launch_bwd<D, false, true>(m, p0, p1, s) : launch_bwd<D, false, false>(m, p0, p1, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+// strides: 24 element strides for {q, k, v, out, dout, dq, dk, dv} x {seq, batch, head}; lse (from the forward) and dvec
+// (scratch): fp32 [B, nh, S_pad]; the rest as for gfs_masked_attention_fwd. dq shares no memory with anything that is read
+// for dk and dv, nor with them: its kernel runs beside theirs.
+int gfs_masked_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout,
+                             const void* lse, void* dvec, void* dq, void* dk, void* dv, const void* mask, int S, int B,
+                             int nh, int nkv, int D, const long long* strides, float scale, float cap, const void* slopes,
+                             void* stream_) {
+  if ((D != 64 && D != 128) || !strides_ok(strides, 24) || nkv <= 0 || nh % nkv != 0) return -1;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+       reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(dq) |
+       reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15)
+    return -2;
+  if (S <= 0 || B <= 0 || nh <= 0) return 0;
+  const int S_pad = (S + 127) / 128 * 128;
+  if (static_cast<long long>(S_pad) * B * nh > 0x3fffffffll) return -1;   // 32-bit row numbers in the pre-pass
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  const long long *sq = strides, *sk = strides + 3, *sv = strides + 6, *so = strides + 9, *sdo = strides + 12,
+                  *sdq = strides + 15, *sdk = strides + 18, *sdv = strides + 21;
+  const int* m = static_cast<const int*>(mask);
+  const size_t n = static_cast<size_t>(B) * S_pad;
+  MaskedBwdParams p = {};
+  p.mask = MaskView{m, m + n, m + 2 * n, m + 3 * n, m + 4 * n};
+  {
+    const long long rows = static_cast<long long>(S_pad) * B * nh;
+    const int threads = 256;
+    const int rows_per_block = threads / (D >> 3) * DVEC_ROWS;
+    const dim3 grid(static_cast<unsigned>((rows + rows_per_block - 1) / rows_per_block));
+    gfs_host::launch_pdl(masked_dvec_kernel, grid, dim3(threads), 0, stream, static_cast<const __nv_bfloat16*>(dout),
+                         static_cast<const __nv_bfloat16*>(out), static_cast<float*>(dvec), p.mask.first, p.mask.last, S,
+                         S_pad, B, nh, D, sdo[0], sdo[1], sdo[2], so[0], so[1], so[2], so[0] < so[2] ? 1 : 0);
+    if (cudaGetLastError() != cudaSuccess) return -11;
+  }
+  const BwdMaps maps{make_map(q, D, S, nh, B, sq, 128), make_map(k, D, S, nkv, B, sk, 128),
+                     make_map(v, D, S, nkv, B, sv, 128), make_map(dout, D, S, nh, B, sdo, 128),
+                     make_map(q, D, S, nh, B, sq, 64), make_map(k, D, S, nkv, B, sk, 64),
+                     make_map(v, D, S, nkv, B, sv, 64), make_map(dout, D, S, nh, B, sdo, 64)};
+  if (!maps.q128 || !maps.k128 || !maps.v128 || !maps.do128 || !maps.q64 || !maps.k64 || !maps.v64 || !maps.do64) return -3;
+  p.lse = static_cast<const float*>(lse);
+  p.dvec = static_cast<const float*>(dvec);
+  p.S = S; p.S_pad = S_pad; p.B = B; p.nh = nh; p.group = nh / nkv; p.scale = scale;
+  p.score.sl2 = cap > 0.f ? 2.f * scale * LOG2E_F / cap : scale * LOG2E_F;
+  p.score.cap2 = cap * LOG2E_F;
+  p.score.slopes = static_cast<const float*>(slopes);
+  p.status = gfs_host::status_words();
+  MaskedBwdParams p0 = p, p1 = p;
+  p0.out1 = static_cast<__nv_bfloat16*>(dk); p0.o1_ss = sdk[0]; p0.o1_bs = sdk[1]; p0.o1_hs = sdk[2];
+  p0.out2 = static_cast<__nv_bfloat16*>(dv); p0.o2_ss = sdv[0]; p0.o2_bs = sdv[1]; p0.o2_hs = sdv[2];
+  p1.out1 = static_cast<__nv_bfloat16*>(dq); p1.o1_ss = sdq[0]; p1.o1_bs = sdq[1]; p1.o1_hs = sdq[2];
+  return D == 64 ? launch_bwd_scores<64>(maps, p0, p1, cap > 0.f, stream)
+                 : launch_bwd_scores<128>(maps, p0, p1, cap > 0.f, stream);
+}
+
+}  // extern "C"
