@@ -401,7 +401,7 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
           *reinterpret_cast<uint4*>(dst + 32 * c + e) = make_uint4(two(c, e), two(c, e + 2), two(c, e + 4), two(c, e + 6));
       }
     }
-    if (half == 0)
+    if (half == 0 && p.lse != nullptr)
       p.lse[static_cast<size_t>(bh) * p.S_pad + row] = l > 0.f ? m * k + log2f(l) : (l == 0.f ? INFINITY : l);
   }
 
@@ -453,7 +453,7 @@ int gfs_attention_mask(const void* ids, int ids64, const void* prefix, int B, in
 }
 
 // q [B, nh, S, D], k and v [B, nkv, S, D], out like q; strides: 12 element strides {q, k, v, out} x {seq, batch, head}.
-// mask: from gfs_attention_mask, of the same B and S. lse: fp32 [B, nh, S_pad], base 2. cap 0: scores as they are.
+// mask: from gfs_attention_mask, of the same B and S. lse: fp32 [B, nh, S_pad], base 2, or null (no backward will follow). cap 0: scores as they are.
 // slopes: fp32 [nh] or null.
 int gfs_masked_attention_fwd(const void* q, const void* k, const void* v, void* out, void* lse, const void* mask, int S,
                              int B, int nh, int nkv, int D, const long long* strides, float scale, float cap,

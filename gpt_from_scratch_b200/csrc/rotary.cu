@@ -164,141 +164,192 @@ __device__ __forceinline__ float group_sum(float v) {
 }
 
 constexpr int ROT_THREADS = 256;
-constexpr int ROT_ROWS = 4;      // rows of one token that a group takes together (forward)
-constexpr int ROT_BWD_ROWS = 2;
+constexpr int ROT_WARPS = ROT_THREADS / 32;
 
-// Forward (and the rotation's own backward). A work item is ROT_ROWS heads of a token.
+// A work item is a warp's: up to STEPS * 32 / LANES heads of one kind (q's, k's or v's) of a token. In a step the groups of the
+// warp have neighbouring heads, so a step's load is contiguous; all steps' loads are issued before the first is used.
+template <int LANES, int STEPS>
+struct Items {
+  static constexpr int GROUPS = 32 / LANES;
+  static constexpr int ROWS = GROUPS * STEPS;
+  static constexpr int of(int heads) { return (heads + ROWS - 1) / ROWS; }
+};
+template <typename T>
+constexpr int bwd_steps() { return sizeof(T) == 2 ? 4 : 2; }   // two inputs of up to 16 (32-bit types: 32) bytes a lane and step
+constexpr int FWD_STEPS = 4;
+
+// f32x2 lanes of a vector: eight elements as four pairs.
+__device__ __forceinline__ void to_pairs(const float (&f)[8], uint64_t (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = pack_f32x2(f[2 * i], f[2 * i + 1]);
+}
+__device__ __forceinline__ float pair_sum(uint64_t v) {
+  const float2 f = unpack_f32x2(v);
+  return f.x + f.y;
+}
+
+// Forward (and the rotation's own backward).
 template <typename T, int LANES, bool HALF, bool NORM>
 __global__ void __launch_bounds__(ROT_THREADS)
-rotary_kernel(const RotaryArgs a, unsigned n_items, unsigned items_per_token) {
+rotary_kernel(const RotaryArgs a, unsigned n_items, unsigned items_per_token, int items_q) {
   pdl_wait();
   pdl_trigger();
+  using I = Items<LANES, FWD_STEPS>;
+  const unsigned item = blockIdx.x * ROT_WARPS + (threadIdx.x >> 5);
+  if (item >= n_items) return;
+  const int group = (threadIdx.x & 31) / LANES;
   const int e0 = (threadIdx.x & (LANES - 1)) * 8;
-  unsigned item = blockIdx.x * (ROT_THREADS / LANES) + threadIdx.x / LANES;
-  const bool live = item < n_items && e0 < a.D;     // lanes past D, groups past the end: no accesses, but every shuffle
-  item = min(item, n_items - 1);
+  const bool lane_on = e0 < a.D;
   const unsigned token = item / items_per_token;
-  const int h0 = static_cast<int>(item - token * items_per_token) * ROT_ROWS;
+  int c = static_cast<int>(item - token * items_per_token);
   const int s = static_cast<int>(token / a.B), b = static_cast<int>(token % a.B);
-  const int heads = a.n1 + a.n2;
-  Vec8<T> x[ROT_ROWS];
+  const bool is_q = c < items_q;
+  if (!is_q) c -= items_q;
+  const int heads = is_q ? a.n1 : a.n2, h0 = c * I::ROWS + group;
+  const T* x = static_cast<const T*>(a.x.p) + a.x.at(s, b, (is_q ? 0 : a.n1) + h0) + e0;
+  Vec8<T> in[FWD_STEPS];
 #pragma unroll
-  for (int i = 0; i < ROT_ROWS; ++i)
-    if (live && h0 + i < heads) x[i] = load_vec(static_cast<const T*>(a.x.p) + a.x.at(s, b, h0 + i) + e0);
-  Turn<HALF> t = {};
-  if (live) t = load_turn<HALF>(a, table_row(a, s, b), e0);
-#pragma unroll
-  for (int i = 0; i < ROT_ROWS; ++i) {
-    const int h = h0 + i;
-    const bool on = live && h < heads;
+  for (int i = 0; i < FWD_STEPS; ++i)
+    if (lane_on && h0 + i * I::GROUPS < heads) in[i] = load_vec(x + i * I::GROUPS * a.x.hs);
+  uint64_t w[4];
+  if (NORM) {
     float f[8] = {};
-    if (on) to_floats(x[i], f);
+    if (lane_on) to_floats(load_vec(static_cast<const T*>(is_q ? a.w1 : a.w2) + e0), f);
+    to_pairs(f, w);
+  }
+  Turn<HALF> t = {};
+  if (lane_on) t = load_turn<HALF>(a, table_row(a, s, b), e0);
+  const Part& out = is_q ? a.y1 : a.y2;
+  T* y = static_cast<T*>(out.p) + out.at(s, b, h0) + e0;
+#pragma unroll
+  for (int i = 0; i < FWD_STEPS; ++i) {
+    if (h0 - group + i * I::GROUPS >= heads) break;      // the whole warp is past the last head
+    const bool on = lane_on && h0 + i * I::GROUPS < heads;
+    float f[8] = {};
+    if (on) to_floats(in[i], f);
     if (NORM) {
-      float ss = 0.f;
+      uint64_t v[4], ss = 0;
+      to_pairs(f, v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
-      const float rstd = rsqrtf(group_sum<LANES>(ss) / static_cast<float>(a.D) + a.eps);
-      if (on) {
-        float w[8];
-        to_floats(load_vec(static_cast<const T*>(h < a.n1 ? a.w1 : a.w2) + e0), w);
+      for (int e = 0; e < 4; ++e) ss = fma_f32x2(v[e], v[e], ss);
+      const float rstd = rsqrtf(group_sum<LANES>(pair_sum(ss)) / static_cast<float>(a.D) + a.eps);
+      const uint64_t r2 = pack_f32x2(rstd, rstd);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= rstd * w[e];
+      for (int e = 0; e < 4; ++e) {
+        const float2 z = unpack_f32x2(mul_f32x2(mul_f32x2(v[e], r2), w[e]));
+        f[2 * e] = z.x;
+        f[2 * e + 1] = z.y;
       }
     }
     rotate<HALF, LANES>(f, t, e0, a.R);
-    if (on) {
-      if (h < a.n1) store_vec(static_cast<T*>(a.y1.p) + a.y1.at(s, b, h) + e0, f);
-      else store_vec(static_cast<T*>(a.y2.p) + a.y2.at(s, b, h - a.n1) + e0, f);
-    }
+    if (on) store_vec(y + i * I::GROUPS * out.hs, f);
   }
 }
 
-// Backward of norm and rotation, of q's and k's heads; v's gradient is copied into its place. A grid of fixed size
-// strides over the items; the weights' gradients stay in registers until the end: a sum per block, added up
-// in a fixed order by qk_norm_dw_kernel.
+// Backward of norm and rotation, of q's and k's heads; v's gradient is copied into its place. A grid of the warps that fit
+// strides over the items; the weights' gradients stay in registers until the end: a sum per block, added up in a fixed
+// order by qk_norm_dw_kernel.
 template <typename T, int LANES, bool HALF, bool NORM>
-__global__ void __launch_bounds__(ROT_THREADS)
-qk_norm_rope_bwd_kernel(const RotaryArgs a, unsigned n_items, unsigned items_per_token) {
+__global__ void __launch_bounds__(ROT_THREADS, 2)
+qk_norm_rope_bwd_kernel(const RotaryArgs a, unsigned n_items, unsigned items_per_token, int items_q, int items_k) {
   pdl_wait();
   pdl_trigger();
-  constexpr int GROUPS = ROT_THREADS / LANES;
+  constexpr int STEPS = bwd_steps<T>();
+  using I = Items<LANES, STEPS>;
+  const int group = (threadIdx.x & 31) / LANES;
   const int e0 = (threadIdx.x & (LANES - 1)) * 8;
-  const int heads = a.n1 + a.n2 + a.n3;
-  float dw1[8] = {}, dw2[8] = {};
-  // every group of a warp makes as many rounds as the others: the shuffles are the whole warp's
-  for (unsigned base = blockIdx.x * GROUPS; base < n_items; base += gridDim.x * GROUPS) {
-    const unsigned item_ = base + threadIdx.x / LANES;
-    const bool live = item_ < n_items && e0 < a.D;
-    const unsigned item = min(item_, n_items - 1);
+  const bool lane_on = e0 < a.D;
+  const float inv_D = 1.f / static_cast<float>(a.D);
+  uint64_t dw1[4] = {}, dw2[4] = {};
+  for (unsigned item = blockIdx.x * ROT_WARPS + (threadIdx.x >> 5); item < n_items; item += gridDim.x * ROT_WARPS) {
     const unsigned token = item / items_per_token;
-    const int h0 = static_cast<int>(item - token * items_per_token) * ROT_BWD_ROWS;
+    int c = static_cast<int>(item - token * items_per_token);
     const int s = static_cast<int>(token / a.B), b = static_cast<int>(token % a.B);
-    Vec8<T> x[ROT_BWD_ROWS], g[ROT_BWD_ROWS];
+    const int kind = c < items_q ? 0 : (c < items_q + items_k ? 1 : 2);
+    c -= kind == 0 ? 0 : (kind == 1 ? items_q : items_q + items_k);
+    const int heads = kind == 0 ? a.n1 : (kind == 1 ? a.n2 : a.n3), h0 = c * I::ROWS + group;
+    const int head0 = (kind == 0 ? 0 : (kind == 1 ? a.n1 : a.n1 + a.n2)) + h0;
+    const Part& from = kind == 0 ? a.y1 : (kind == 1 ? a.y2 : a.y3);
+    const T* g = static_cast<const T*>(from.p) + from.at(s, b, h0) + e0;
+    const T* x = static_cast<const T*>(a.x.p) + a.x.at(s, b, head0) + e0;
+    T* dx = static_cast<T*>(a.dx.p) + a.dx.at(s, b, head0) + e0;
+    Vec8<T> gv[STEPS], xv[STEPS];
 #pragma unroll
-    for (int i = 0; i < ROT_BWD_ROWS; ++i) {
-      const int h = h0 + i;
-      if (live && h < heads) {
-        if (h < a.n1) g[i] = load_vec(static_cast<const T*>(a.y1.p) + a.y1.at(s, b, h) + e0);
-        else if (h < a.n1 + a.n2) g[i] = load_vec(static_cast<const T*>(a.y2.p) + a.y2.at(s, b, h - a.n1) + e0);
-        else g[i] = load_vec(static_cast<const T*>(a.y3.p) + a.y3.at(s, b, h - a.n1 - a.n2) + e0);
-        if (NORM && h < a.n1 + a.n2) x[i] = load_vec(static_cast<const T*>(a.x.p) + a.x.at(s, b, h) + e0);
+    for (int i = 0; i < STEPS; ++i)
+      if (lane_on && h0 + i * I::GROUPS < heads) {
+        gv[i] = load_vec(g + i * I::GROUPS * from.hs);
+        if (NORM && kind != 2) xv[i] = load_vec(x + i * I::GROUPS * a.x.hs);
       }
+    if (kind == 2) {
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i)
+        if (lane_on && h0 + i * I::GROUPS < heads)
+#pragma unroll
+          for (int u = 0; u < static_cast<int>(sizeof(Vec8<T>) / 16); ++u)
+            reinterpret_cast<uint4*>(dx + i * I::GROUPS * a.dx.hs)[u] = reinterpret_cast<const uint4*>(&gv[i])[u];
+      continue;
+    }
+    uint64_t w[4], dw[4] = {};
+    if (NORM) {
+      float f[8] = {};
+      if (lane_on) to_floats(load_vec(static_cast<const T*>(kind == 0 ? a.w1 : a.w2) + e0), f);
+      to_pairs(f, w);
     }
     Turn<HALF> t = {};
-    if (live && h0 < a.n1 + a.n2) t = load_turn<HALF>(a, table_row(a, s, b), e0);
+    if (lane_on) t = load_turn<HALF>(a, table_row(a, s, b), e0);
 #pragma unroll
-    for (int i = 0; i < ROT_BWD_ROWS; ++i) {
-      const int h = h0 + i;
-      const bool on = live && h < heads;
-      const bool turn = on && h < a.n1 + a.n2;
-      float dz[8] = {};
-      if (on) to_floats(g[i], dz);
-      float raw[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) raw[e] = dz[e];
-      rotate<HALF, LANES>(dz, t, e0, a.R);
+    for (int i = 0; i < STEPS; ++i) {
+      if (h0 - group + i * I::GROUPS >= heads) break;
+      const bool on = lane_on && h0 + i * I::GROUPS < heads;
+      float f[8] = {};
+      if (on) to_floats(gv[i], f);
+      rotate<HALF, LANES>(f, t, e0, a.R);
       if (NORM) {
-        float f[8] = {}, w[8] = {};
-        if (turn) {
-          to_floats(x[i], f);
-          to_floats(load_vec(static_cast<const T*>(h < a.n1 ? a.w1 : a.w2) + e0), w);
-        }
-        float ss = 0.f, dot = 0.f;
+        uint64_t dz[4], v[4], zw[4], ss = 0, dot = 0;
+        to_pairs(f, dz);
+        float xf[8] = {};
+        if (on) to_floats(xv[i], xf);
+        to_pairs(xf, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          ss += f[e] * f[e];
-          dot += dz[e] * w[e] * f[e];
+        for (int e = 0; e < 4; ++e) {
+          zw[e] = mul_f32x2(dz[e], w[e]);
+          ss = fma_f32x2(v[e], v[e], ss);
+          dot = fma_f32x2(zw[e], v[e], dot);
         }
-        ss = group_sum<LANES>(ss);
-        dot = group_sum<LANES>(dot);
-        const float rstd = rsqrtf(ss / static_cast<float>(a.D) + a.eps);
-        const float m = dot * rstd * rstd / static_cast<float>(a.D);      // mean(dz w n) rstd
-        if (turn) {
+        const float rstd = rsqrtf(group_sum<LANES>(pair_sum(ss)) * inv_D + a.eps);
+        const float m = group_sum<LANES>(pair_sum(dot)) * rstd * rstd * inv_D;      // mean(dz w n) rstd
+        const uint64_t r2 = pack_f32x2(rstd, rstd), m2 = pack_f32x2(-m, -m);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float n = f[e] * rstd;
-            if (h < a.n1) dw1[e] += dz[e] * n;
-            else dw2[e] += dz[e] * n;
-            dz[e] = rstd * dz[e] * w[e] - n * m;
-          }
+        for (int e = 0; e < 4; ++e) {
+          const uint64_t n = mul_f32x2(v[e], r2);
+          dw[e] = fma_f32x2(dz[e], n, dw[e]);
+          const float2 o = unpack_f32x2(fma_f32x2(n, m2, mul_f32x2(zw[e], r2)));
+          f[2 * e] = o.x;
+          f[2 * e + 1] = o.y;
         }
       }
-      if (on) {
-        if (!turn) {
+      if (on) store_vec(dx + i * I::GROUPS * a.dx.hs, f);
+    }
+    if (NORM) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) dz[e] = raw[e];
-        }
-        store_vec(static_cast<T*>(a.dx.p) + a.dx.at(s, b, h) + e0, dz);
+      for (int e = 0; e < 4; ++e) {
+        if (kind == 0) dw1[e] = add_f32x2(dw1[e], dw[e]);
+        else dw2[e] = add_f32x2(dw2[e], dw[e]);
       }
     }
   }
   if (NORM) {
+    constexpr int GROUPS = ROT_THREADS / LANES;
     __shared__ float part[GROUPS][LANES * 8];
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) part[threadIdx.x / LANES][e0 + e] = which == 0 ? dw1[e] : dw2[e];
+      for (int e = 0; e < 4; ++e) {
+        const float2 d = unpack_f32x2(which == 0 ? dw1[e] : dw2[e]);
+        part[threadIdx.x / LANES][e0 + 2 * e] = d.x;
+        part[threadIdx.x / LANES][e0 + 2 * e + 1] = d.y;
+      }
       __syncthreads();
       for (int d = threadIdx.x; d < a.D; d += ROT_THREADS) {
         float sum = 0.f;
@@ -476,19 +527,19 @@ int launch_forward(const RotaryArgs& a, bool vec, cudaStream_t stream) {
     const unsigned blocks = std::min<unsigned>((rows + 7) / 8, gfs_host::sm_count() * 32);
     gfs_host::launch_pdl(rotary_any_kernel<T, HALF, NORM>, dim3(blocks), dim3(ROT_THREADS), 0, stream, a, rows);
   } else {
-    const unsigned per = (heads + ROT_ROWS - 1) / ROT_ROWS;
-    const unsigned items = static_cast<unsigned>(tokens) * per;
     const int lanes = a.D <= 64 ? 8 : (a.D <= 128 ? 16 : 32);
-    const unsigned groups = ROT_THREADS / lanes;
-    const dim3 grid((items + groups - 1) / groups);
+    const int rows = FWD_STEPS * 32 / lanes;
+    const int items_q = (a.n1 + rows - 1) / rows, per = items_q + (a.n2 + rows - 1) / rows;
+    const unsigned items = static_cast<unsigned>(tokens) * per;
     auto kern = lanes == 8 ? rotary_kernel<T, 8, HALF, NORM>
                            : (lanes == 16 ? rotary_kernel<T, 16, HALF, NORM> : rotary_kernel<T, 32, HALF, NORM>);
-    gfs_host::launch_pdl(kern, grid, dim3(ROT_THREADS), 0, stream, a, items, per);
+    gfs_host::launch_pdl(kern, dim3((items + ROT_WARPS - 1) / ROT_WARPS), dim3(ROT_THREADS), 0, stream, a, items,
+                         static_cast<unsigned>(per), items_q);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 
-int bwd_blocks() { return gfs_host::sm_count() * 4; }
+int bwd_blocks() { return gfs_host::sm_count() * 2; }   // what is resident
 
 template <typename T, bool HALF, bool NORM>
 int launch_backward(const RotaryArgs& a, bool vec, T* dw1, T* dw2, cudaStream_t stream) {
@@ -501,15 +552,17 @@ int launch_backward(const RotaryArgs& a, bool vec, T* dw1, T* dw2, cudaStream_t 
     blocks = std::min<unsigned>((rows + 7) / 8, bwd_blocks());
     gfs_host::launch_pdl(qk_norm_rope_bwd_any_kernel<T, HALF, NORM>, dim3(blocks), dim3(ROT_THREADS), 0, stream, a, rows);
   } else {
-    const unsigned per = (heads + ROT_BWD_ROWS - 1) / ROT_BWD_ROWS;
-    const unsigned items = static_cast<unsigned>(tokens) * per;
     const int lanes = a.D <= 64 ? 8 : (a.D <= 128 ? 16 : 32);
-    const unsigned groups = ROT_THREADS / lanes;
-    blocks = std::min<unsigned>((items + groups - 1) / groups, bwd_blocks());
+    const int rows = bwd_steps<T>() * 32 / lanes;
+    const int items_q = (a.n1 + rows - 1) / rows, items_k = (a.n2 + rows - 1) / rows;
+    const int per = items_q + items_k + (a.n3 + rows - 1) / rows;
+    const unsigned items = static_cast<unsigned>(tokens) * per;
+    blocks = std::min<unsigned>((items + ROT_WARPS - 1) / ROT_WARPS, bwd_blocks());
     auto kern = lanes == 8 ? qk_norm_rope_bwd_kernel<T, 8, HALF, NORM>
                            : (lanes == 16 ? qk_norm_rope_bwd_kernel<T, 16, HALF, NORM>
                                           : qk_norm_rope_bwd_kernel<T, 32, HALF, NORM>);
-    gfs_host::launch_pdl(kern, dim3(blocks), dim3(ROT_THREADS), 0, stream, a, items, per);
+    gfs_host::launch_pdl(kern, dim3(blocks), dim3(ROT_THREADS), 0, stream, a, items, static_cast<unsigned>(per), items_q,
+                         items_k);
   }
   if (cudaGetLastError() != cudaSuccess) return -11;
   if (NORM) {

@@ -199,6 +199,16 @@ def on_device(t: torch.Tensor):
     return _NULL_RANGE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
+def first_order(backward):
+    """A ``Function.backward`` that autograd cannot differentiate again: ``once_differentiable`` where a graph of the
+    backward is being made, the bare function (8 us less) where none is."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 def ptr(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 

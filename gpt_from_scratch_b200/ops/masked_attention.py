@@ -8,37 +8,54 @@ block that it hides.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
-from dataclasses import dataclass
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
-_Strides12, _Strides24 = ctypes.c_longlong * 12, ctypes.c_longlong * 24
 
-
-@dataclass(frozen=True)
 class AttentionMask:
     """What :func:`attention_mask` returns. ``first``, ``last``: int32 ``[B, S]``, query s sees the keys ``[first, last)`` (none:
     padding); ``positions``: int32 ``[B, S]``, the place of every token in its document (for
     :func:`~gpt_from_scratch_b200.ops.rope.rotary`)."""
-    batch: int
-    seq_len: int
-    first: torch.Tensor
-    last: torch.Tensor
-    positions: torch.Tensor
-    buffer: torch.Tensor | None = None      # CUDA: what the kernels read (see gfs_attention_mask)
+    __slots__ = ("batch", "seq_len", "device", "buffer", "_parts")
+
+    def __init__(self, batch: int, seq_len: int, device: torch.device, buffer: torch.Tensor | None = None, parts=None):
+        self.batch, self.seq_len, self.device = batch, seq_len, device
+        self.buffer = buffer        # CUDA: what the kernels read (gfs_attention_mask); its parts are cut out when asked for
+        self._parts = parts
+
+    def _part(self, i: int) -> torch.Tensor:
+        if self._parts is not None:
+            return self._parts[i]
+        B, S = self.batch, self.seq_len
+        S_pad = _pad128(S)
+        if i == 2:
+            return self.buffer.as_strided((B, S), (S, 1), 4 * B * S_pad + B)
+        return self.buffer.as_strided((B, S), (S_pad, 1), i * B * S_pad)
 
     @property
-    def device(self) -> torch.device:
-        return self.first.device
+    def first(self) -> torch.Tensor:
+        return self._part(0)
+
+    @property
+    def last(self) -> torch.Tensor:
+        return self._part(1)
+
+    @property
+    def positions(self) -> torch.Tensor:
+        return self._part(2)
 
     def visible(self) -> torch.Tensor:
         """bool ``[B, S, S]``, query by key."""
         at = torch.arange(self.seq_len, device=self.device)
         return (at >= self.first.unsqueeze(-1)) & (at < self.last.unsqueeze(-1))
+
+
+def _pad128(S: int) -> int:
+    return (S + 127) // 128 * 128
 
 
 def _mask_reference(batch, seq_len, causal, ids, prefix, window, device):
@@ -61,7 +78,7 @@ def _mask_reference(batch, seq_len, causal, ids, prefix, window, device):
         first = torch.maximum(first, at - window + 1)
     if ids is not None:
         first, last = torch.where(ids < 0, start, first), torch.where(ids < 0, start, last)
-    return AttentionMask(batch, S, first.int(), last.int(), (at - start).int())
+    return AttentionMask(batch, S, device, parts=(first.int(), last.int(), (at - start).int()))
 
 
 def attention_mask(batch: int, seq_len: int, causal: bool = True, document_ids: torch.Tensor | None = None,
@@ -96,15 +113,12 @@ def attention_mask(batch: int, seq_len: int, causal: bool = True, document_ids: 
     ids = None if document_ids is None else document_ids.contiguous()
     prefix = None if prefix_mask is None else prefix_mask.contiguous()
     B, S = batch, seq_len
-    S_pad = (S + 127) // 128 * 128
-    n = B * S_pad
-    buffer = torch.empty(4 * n + B + B * S, dtype=torch.int32, device=device)
+    buffer = torch.empty(4 * B * _pad128(S) + B + B * S, dtype=torch.int32, device=device)
     with _lib.on_device(buffer), _lib.nvtx("attention_mask"):
         rc = _lib.lib().gfs_attention_mask(_lib.ptr(ids), ids is not None and ids.dtype == torch.int64, _lib.ptr(prefix), B,
                                            S, causal, min(window or 0, 0x7fffffff), buffer.data_ptr(), _lib.stream_ptr())
     _lib.check(rc, "gfs_attention_mask")
-    return AttentionMask(B, S, buffer.as_strided((B, S), (S_pad, 1), 0), buffer.as_strided((B, S), (S_pad, 1), n),
-                         buffer.as_strided((B, S), (S, 1), 4 * n + B), buffer)
+    return AttentionMask(B, S, device, buffer)
 
 
 def masked_attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: AttentionMask, softcap: float = 0.0,
@@ -125,56 +139,75 @@ def masked_attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
     return torch.matmul(p, v).to(q.dtype)
 
 
-def _strides(t: torch.Tensor) -> tuple[int, int, int]:
+@functools.lru_cache(maxsize=1024)
+def _strides(shape, stride) -> tuple[int, int, int]:
     """Element strides (sequence, batch, head) of a ``[B, heads, S, D]`` tensor; those of single entries, which lead
     nowhere, are given as the kernels want them."""
-    b, h, s, _ = t.stride()
-    nb, nh, ns, d = t.shape
+    (nb, nh, ns, d), (b, h, s, _) = shape, stride
     return s if ns > 1 else d, b if nb > 1 else d, h if nh > 1 else d
+
+
+@functools.lru_cache(maxsize=1024)
+def _stride_array(*layouts):
+    """ctypes array of the strides of tensors given as shape, stride, shape, stride, ..."""
+    flat = [n for shape, stride in zip(layouts[::2], layouts[1::2]) for n in _strides(shape, stride)]
+    return (ctypes.c_longlong * len(flat))(*flat)
+
+
+@functools.lru_cache(maxsize=1024)
+def _steps_of_16_bytes(shape, stride) -> bool:
+    return stride[3] == 1 and all(s > 0 and s % 8 == 0 for s in _strides(shape, stride))
 
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself if the kernels can read its layout (16-byte steps, no broadcast dimensions), else a contiguous copy."""
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s > 0 and s % 8 == 0 for s in _strides(t)):
+    if not t.data_ptr() % 16 and _steps_of_16_bytes(t.shape, t.stride()):
         return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def _forward(q, k, v, buffer, slopes, softcap: float, scale: float, want_lse: bool):
+    B, nh, S, D = q.shape
+    out = torch.empty_like(q)
+    lse = torch.empty((B, nh, _pad128(S)), dtype=torch.float32, device=q.device) if want_lse else None
+    kv = k.shape
+    st = _stride_array(q.shape, q.stride(), kv, k.stride(), kv, v.stride(), q.shape, out.stride())
+    with _lib.on_device(q), _lib.nvtx("masked_attention_fwd"):
+        rc = _lib.lib().gfs_masked_attention_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _lib.ptr(lse),
+                                                 buffer.data_ptr(), S, B, nh, kv[1], D, st, scale, softcap,
+                                                 _lib.ptr(slopes), _lib.stream_ptr())
+    _lib.check(rc, "gfs_masked_attention_fwd")
+    return out, lse
 
 
 class _MaskedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, buffer, slopes, softcap, scale):
-        B, nh, S, D = q.shape
-        nkv = k.shape[1]
         q, k, v = _readable(q), _readable(k), _readable(v)
-        out = torch.empty_like(q)
-        lse = torch.empty((B, nh, (S + 127) // 128 * 128), dtype=torch.float32, device=q.device)
-        st = _Strides12(*_strides(q), *_strides(k), *_strides(v), *_strides(out))
-        with _lib.on_device(q), _lib.nvtx("masked_attention_fwd"):
-            rc = _lib.lib().gfs_masked_attention_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                                     lse.data_ptr(), buffer.data_ptr(), S, B, nh, nkv, D, st, scale,
-                                                     softcap, _lib.ptr(slopes), _lib.stream_ptr())
-        _lib.check(rc, "gfs_masked_attention_fwd")
+        out, lse = _forward(q, k, v, buffer, slopes, softcap, scale, True)
         ctx.save_for_backward(q, k, v, out, lse, buffer, slopes)
         ctx.args = (softcap, scale)
         return out
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, dout):
         q, k, v, out, lse, buffer, slopes = ctx.saved_tensors
         softcap, scale = ctx.args
-        B, nh, S, D = q.shape
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         if q.numel() == 0:
             return dq, dk, dv, None, None, None, None
+        B, nh, S, D = shape = q.shape
+        kv = k.shape
         dout = _readable(dout)
         dvec = torch.empty_like(lse)
-        st = _Strides24(*(n for t in (q, k, v, out, dout, dq, dk, dv) for n in _strides(t)))
+        st = _stride_array(shape, q.stride(), kv, k.stride(), kv, v.stride(), shape, out.stride(), shape, dout.stride(), shape,
+                           dq.stride(), kv, dk.stride(), kv, dv.stride())
         with _lib.on_device(q), _lib.nvtx("masked_attention_bwd"):
             rc = _lib.lib().gfs_masked_attention_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                                                      dout.data_ptr(), lse.data_ptr(), dvec.data_ptr(), dq.data_ptr(),
-                                                     dk.data_ptr(), dv.data_ptr(), buffer.data_ptr(), S, B, nh, k.shape[1],
-                                                     D, st, scale, softcap, _lib.ptr(slopes), _lib.stream_ptr())
+                                                     dk.data_ptr(), dv.data_ptr(), buffer.data_ptr(), S, B, nh, kv[1], D,
+                                                     st, scale, softcap, _lib.ptr(slopes), _lib.stream_ptr())
         _lib.check(rc, "gfs_masked_attention_bwd")
         _lib.add_launches(2)  # pre-pass + two main kernels
         return dq, dk, dv, None, None, None, None
@@ -214,6 +247,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
         if q.dtype != torch.bfloat16 or D not in (64, 128):
             raise ValueError(f"masked_attention: no native kernel for {q.dtype} and head_dim {D} (bfloat16 and 64 or 128 have "
                              "one); use masked_attention_reference for others")
-        return _MaskedAttention.apply(q, k, v, mask.buffer, None if alibi_slopes is None else alibi_slopes.contiguous(),
-                                      float(softcap), float(scale))
+        slopes = None if alibi_slopes is None else alibi_slopes.contiguous()
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            return _MaskedAttention.apply(q, k, v, mask.buffer, slopes, float(softcap), float(scale))
+        return _forward(_readable(q), _readable(k), _readable(v), mask.buffer, slopes, float(softcap), float(scale), False)[0]
     return masked_attention_reference(q, k, v, mask, softcap, alibi_slopes, scale)

@@ -7,15 +7,10 @@ once, in the backward too, which recomputes the norm and writes the gradient of 
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .rope import NATIVE_TYPES, check_tables, rotary_reference, rows_of
-
-_Strides3, _Strides15 = ctypes.c_longlong * 3, ctypes.c_longlong * 15
+from .rope import NATIVE_TYPES, check_tables, rotary_reference, rows_of, stride_array
 
 
 def qk_norm_rope_reference(qkv, q_weight, k_weight, cos, sin, num_heads, num_kv_heads, eps=1e-5, positions=None,
@@ -33,54 +28,57 @@ def qk_norm_rope_reference(qkv, q_weight, k_weight, cos, sin, num_heads, num_kv_
     return one(q, q_weight), one(k, k_weight), v
 
 
+def _forward(x, q_weight, k_weight, cos, sin, n1, n2, eps, positions, interleaved):
+    S, B, W = x.shape
+    D = W // (n1 + 2 * n2)
+    q = torch.empty((S, B, n1, D), dtype=x.dtype, device=x.device)
+    k = torch.empty((S, B, n2, D), dtype=x.dtype, device=x.device)
+    ss, bs, _ = x.stride()
+    with _lib.on_device(x), _lib.nvtx("qk_norm_rope"):
+        rc = _lib.lib().gfs_qk_norm_rope_fwd(
+            x.data_ptr(), stride_array((ss, bs, D)), _lib.ptr(q_weight), _lib.ptr(k_weight), q.data_ptr(), k.data_ptr(),
+            cos.data_ptr(), sin.data_ptr(), _lib.ptr(positions), positions is not None and positions.dtype == torch.int64,
+            cos.shape[0], S, B, n1, n2, D, 2 * cos.shape[1], not interleaved, eps, NATIVE_TYPES[x.dtype],
+            _lib.stream_ptr())
+    _lib.check(rc, "gfs_qk_norm_rope_fwd")
+    return q, k, x.as_strided((S, B, n2, D), (ss, bs, D, 1), x.storage_offset() + (n1 + n2) * D)
+
+
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, q_weight, k_weight, cos, sin, n1, n2, eps, positions, interleaved):
-        S, B, W = qkv.shape
-        D = W // (n1 + 2 * n2)
-        x = rows_of(qkv).unflatten(-1, (n1 + 2 * n2, D))
-        q = torch.empty((S, B, n1, D), dtype=x.dtype, device=x.device)
-        k = torch.empty((S, B, n2, D), dtype=x.dtype, device=x.device)
-        with _lib.on_device(x), _lib.nvtx("qk_norm_rope"):
-            rc = _lib.lib().gfs_qk_norm_rope_fwd(
-                x.data_ptr(), _Strides3(*x.stride()[:3]), _lib.ptr(q_weight), _lib.ptr(k_weight), q.data_ptr(),
-                k.data_ptr(), cos.data_ptr(), sin.data_ptr(), _lib.ptr(positions),
-                positions is not None and positions.dtype == torch.int64, cos.shape[0], S, B, n1, n2, D,
-                2 * cos.shape[1], not interleaved, eps, NATIVE_TYPES[x.dtype], _lib.stream_ptr())
-        _lib.check(rc, "gfs_qk_norm_rope_fwd")
         ctx.save_for_backward(qkv, q_weight, k_weight, cos, sin, positions)
-        ctx.args = (n1, n2, D, eps, interleaved)
-        return q, k, x[:, :, n1 + n2:]
+        ctx.args = (n1, n2, eps, interleaved)
+        return _forward(qkv, q_weight, k_weight, cos, sin, n1, n2, eps, positions, interleaved)
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, dq, dk, dv):
         qkv, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        n1, n2, D, eps, interleaved = ctx.args
+        n1, n2, eps, interleaved = ctx.args
         S, B, W = qkv.shape
+        D = W // (n1 + 2 * n2)
         lib = _lib.lib()
-        x = rows_of(qkv).unflatten(-1, (n1 + 2 * n2, D))
         dq, dk, dv = rows_of(dq), rows_of(dk), rows_of(dv)
         dqkv = torch.empty((S, B, W), dtype=qkv.dtype, device=qkv.device)
-        dx = dqkv.unflatten(-1, (n1 + 2 * n2, D))
-        dw1 = dw2 = scratch = None
-        if q_weight is not None:
-            dw1, dw2 = torch.empty_like(q_weight), torch.empty_like(k_weight)
         if qkv.numel() == 0:
             return dqkv, *(None if w is None else torch.zeros_like(w) for w in (q_weight, k_weight)), *[None] * 7
-        with _lib.on_device(x), _lib.nvtx("qk_norm_rope_bwd"):
+        dw1 = dw2 = scratch = None
+        ss, bs, _ = qkv.stride()
+        with _lib.on_device(qkv), _lib.nvtx("qk_norm_rope_bwd"):
             if q_weight is not None:
-                scratch = torch.empty(lib.gfs_qk_norm_rope_scratch(D), dtype=torch.float32, device=x.device)
-            st = _Strides15(*(n for t in (x, dq, dk, dv, dx) for n in t.stride()[:3]))
+                dw1, dw2 = torch.empty_like(q_weight), torch.empty_like(k_weight)
+                scratch = torch.empty(lib.gfs_qk_norm_rope_scratch(D), dtype=torch.float32, device=qkv.device)
+            st = stride_array((ss, bs, D), dq.stride(), dk.stride(), dv.stride(), (B * W, W, D))
             rc = lib.gfs_qk_norm_rope_bwd(
-                x.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dx.data_ptr(), st, _lib.ptr(q_weight),
+                qkv.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dqkv.data_ptr(), st, _lib.ptr(q_weight),
                 _lib.ptr(k_weight), _lib.ptr(dw1), _lib.ptr(dw2), _lib.ptr(scratch), cos.data_ptr(), sin.data_ptr(),
                 _lib.ptr(positions), positions is not None and positions.dtype == torch.int64, cos.shape[0], S, B, n1, n2,
-                D, 2 * cos.shape[1], not interleaved, eps, NATIVE_TYPES[x.dtype], _lib.stream_ptr())
+                D, 2 * cos.shape[1], not interleaved, eps, NATIVE_TYPES[qkv.dtype], _lib.stream_ptr())
         _lib.check(rc, "gfs_qk_norm_rope_bwd")
         if q_weight is not None:
             _lib.add_launches(1)      # the weights' gradients are added up in a launch of their own
-        return dqkv, dw1, dw2, *[None] * 7
+        return dqkv, dw1, dw2, None, None, None, None, None, None, None
 
 
 def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None, cos: torch.Tensor,
@@ -107,7 +105,12 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: tor
         if w is not None and (w.shape != (D,) or w.dtype != qkv.dtype or w.device != qkv.device):
             raise ValueError(f"qk_norm_rope: weights have to be {qkv.dtype} of shape [{D}] on {qkv.device}")
     if qkv.is_cuda:
-        contiguous = (lambda t: None if t is None else t.contiguous())
-        return _QkNormRope.apply(qkv, contiguous(q_weight), contiguous(k_weight), cos.contiguous(), sin.contiguous(),
-                                 num_heads, num_kv_heads, float(eps), contiguous(positions), bool(interleaved))
+        if q_weight is not None:
+            q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
+        args = (rows_of(qkv), q_weight, k_weight, cos.contiguous(), sin.contiguous(), num_heads, num_kv_heads, float(eps),
+                None if positions is None else positions.contiguous(), bool(interleaved))
+        if torch.is_grad_enabled() and (qkv.requires_grad or (q_weight is not None and
+                                                              (q_weight.requires_grad or k_weight.requires_grad))):
+            return _QkNormRope.apply(*args)
+        return _forward(*args)
     return qk_norm_rope_reference(qkv, q_weight, k_weight, cos, sin, num_heads, num_kv_heads, eps, positions, interleaved)

@@ -12,11 +12,11 @@ inside the packed qkv buffer. cos/sin are fp32 ``[S, D/2]`` tables.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -126,7 +126,12 @@ def rope_tables(length: int, rotary_dim: int, base: float = 10000.0, scaling: Ro
 
 NATIVE_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_HEAD_DIM = 256
-_Strides6 = ctypes.c_longlong * 6
+
+
+@functools.lru_cache(maxsize=1024)
+def stride_array(*strides: tuple[int, ...]):
+    """ctypes array of the first three element strides of each tensor."""
+    return (ctypes.c_longlong * (3 * len(strides)))(*(n for st in strides for n in st[:3]))
 
 
 def rows_of(t: torch.Tensor) -> torch.Tensor:
@@ -188,9 +193,9 @@ def _rotary_native(x, cos, sin, positions, interleaved: bool, inverse: bool) -> 
     S, B, nh, D = x.shape
     x = rows_of(x)
     y = torch.empty((S, B, nh, D), dtype=x.dtype, device=x.device)
-    st = _Strides6(*x.stride()[:3], *y.stride()[:3])
     with _lib.on_device(x), _lib.nvtx("rotary"):
-        rc = _lib.lib().gfs_rotary(x.data_ptr(), y.data_ptr(), st, cos.data_ptr(), sin.data_ptr(), _lib.ptr(positions),
+        rc = _lib.lib().gfs_rotary(x.data_ptr(), y.data_ptr(), stride_array(x.stride(), y.stride()), cos.data_ptr(),
+                                   sin.data_ptr(), _lib.ptr(positions),
                                    positions is not None and positions.dtype == torch.int64, cos.shape[0], S, B, nh, D,
                                    2 * cos.shape[1], not interleaved, inverse, NATIVE_TYPES[x.dtype], _lib.stream_ptr())
     _lib.check(rc, "gfs_rotary")
@@ -205,7 +210,7 @@ class _Rotary(torch.autograd.Function):
         return _rotary_native(x, cos, sin, positions, interleaved, False)
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, dy):
         cos, sin, positions = ctx.saved_tensors
         return _rotary_native(dy, cos, sin, positions, ctx.interleaved, True), None, None, None, None
@@ -226,6 +231,8 @@ def rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: tor
     S, B, _, D = x.shape
     check_tables("rotary", x, cos, sin, positions, S, B, D)
     if x.is_cuda:
-        return _Rotary.apply(x, cos.contiguous(), sin.contiguous(),
-                             None if positions is None else positions.contiguous(), interleaved)
+        args = (x, cos.contiguous(), sin.contiguous(), None if positions is None else positions.contiguous(), interleaved)
+        if torch.is_grad_enabled() and x.requires_grad:
+            return _Rotary.apply(*args)
+        return _rotary_native(*args, False)
     return rotary_reference(x, cos, sin, positions, interleaved)
