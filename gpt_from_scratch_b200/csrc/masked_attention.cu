@@ -57,12 +57,35 @@ struct MaskArgs {
   const uint8_t* prefix;    // [B, S] or null
   int ids64, S, S_pad, window, causal;
   int *first, *last, *qfirst, *qlast, *padded, *positions;
+  int4 *plan_q, *plan_k;
 };
+
+// The tiles of a sequence in descending order of the rows between their ends (the work they are): kernels that start the
+// heaviest first end together. Ranks by counting; a longer sequence than fits has enough tiles to even out by itself.
+constexpr int MASK_SORT = 2048;
+__device__ __forceinline__ void sort_tiles(const int* lo, const int* hi, int S, int4* plan, int* weight) {
+  const int n = (S + 127) >> 7;
+  const bool sorted = n <= MASK_SORT;
+  __syncthreads();
+  for (int t = threadIdx.x; t < n; t += MASK_THREADS)
+    if (sorted) weight[t] = hi[min(t * 128 + 127, S - 1)] - lo[t * 128];
+  __syncthreads();
+  for (int t = threadIdx.x; t < n; t += MASK_THREADS) {
+    int rank = n - 1 - t;
+    if (sorted) {
+      rank = 0;
+      const int mine = weight[t];
+      for (int u = 0; u < n; ++u) rank += weight[u] > mine || (weight[u] == mine && u > t);
+    }
+    plan[rank] = make_int4(t, lo[t * 128], hi[min(t * 128 + 127, S - 1)], 0);
+  }
+}
 
 __global__ void __launch_bounds__(MASK_THREADS) attention_mask_kernel(const MaskArgs a) {
   pdl_wait();
   pdl_trigger();
   __shared__ int tmp[32];
+  __shared__ int weight[MASK_SORT];
   const int b = blockIdx.x;
   const size_t row = static_cast<size_t>(b) * a.S;
   const size_t prow = static_cast<size_t>(b) * a.S_pad;
@@ -122,6 +145,9 @@ __global__ void __launch_bounds__(MASK_THREADS) attention_mask_kernel(const Mask
     a.first[prow + i] = a.last[prow + i] = a.qfirst[prow + i] = a.qlast[prow + i] = a.S;
   any = __syncthreads_or(any);
   if (threadIdx.x == 0) a.padded[b] = any;
+  const size_t tiles = static_cast<size_t>(b) * (a.S_pad / 128);
+  sort_tiles(a.first + prow, a.last + prow, a.S, a.plan_q + tiles, weight);
+  sort_tiles(a.qfirst + prow, a.qlast + prow, a.S, a.plan_k + tiles, weight);
 }
 
 // ---------------------------------------------------------------------------
@@ -200,15 +226,16 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
   WaitCtx wctx{abort_flag, p.status, GFS_WAIT_LIMIT_NS};
 
   const int BH = p.B * p.nh;
-  const int qt = n_tiles - 1 - static_cast<int>(blockIdx.x / BH);     // the last tiles have the most keys: first
+  const int level = static_cast<int>(blockIdx.x / BH);                // the tiles that see the most keys come first
   const int bh = static_cast<int>(blockIdx.x % BH);
   const int b = bh / p.nh, h = bh % p.nh, kvh = h / p.group;
+  const TilePlan plan = load_plan(p.mask.plan_q + static_cast<size_t>(b) * n_tiles + level);
   const int* first = p.mask.first + static_cast<size_t>(b) * p.S_pad;
   const int* last = p.mask.last + static_cast<size_t>(b) * p.S_pad;
-  const int row_a = qt * 128, row_z = min(row_a + 127, p.S - 1);
+  const int row_a = plan.tile * 128, row_z = min(row_a + 127, p.S - 1);
   // blocks [j0, j1) of 128 keys; at least one, which may be masked whole
-  const int j0 = first[row_a] >> 7;
-  const int j1 = max(j0 + 1, (last[row_z] + 127) >> 7);
+  const int j0 = plan.lo >> 7;
+  const int j1 = max(j0 + 1, (plan.hi + 127) >> 7);
 
   if (warp == 0) {
     if (lane == 0) {
@@ -437,19 +464,27 @@ extern "C" {
 // The mask of B sequences of S tokens. ids (int32, or int64 with ids64; null: one document): a run of equal numbers is a
 // document, one of negative numbers padding. prefix (bytes; null: none): the leading tokens of a document that are
 // marked are seen by all of it. causal 0: every token sees its whole document. window (0: none): a query sees no key
-// more than window - 1 tokens back. out: int32, [first | last | qfirst | qlast] of [B, S_pad] each, [B] padded, then
-// positions [B, S], the place of every token in its document.
+// more than window - 1 tokens back. out: int32, laid out as masked_attention.cuh says (gfs_attention_mask_layout), 16-byte
+// aligned.
 int gfs_attention_mask(const void* ids, int ids64, const void* prefix, int B, int S, int causal, int window, void* out,
                        void* stream) {
   if (S < 0 || B < 0 || window < 0 || (!causal && (window > 0 || prefix != nullptr)) || S > 0x7fffff00) return -1;
   if (S == 0 || B == 0) return 0;
-  const int S_pad = (S + 127) / 128 * 128;
+  if (reinterpret_cast<uintptr_t>(out) & 15) return -2;
   int* o = static_cast<int*>(out);
-  const size_t n = static_cast<size_t>(B) * S_pad;
-  const MaskArgs a{ids, static_cast<const uint8_t*>(prefix), ids64, S, S_pad, window > S ? 0 : window, causal,
-                   o, o + n, o + 2 * n, o + 3 * n, o + 4 * n, o + 4 * n + B};
+  const MaskLayout l = mask_layout(B, S);
+  const MaskArgs a{ids, static_cast<const uint8_t*>(prefix), ids64, S, (S + 127) / 128 * 128, window > S ? 0 : window, causal,
+                   o + l.first, o + l.last, o + l.qfirst, o + l.qlast, o + l.padded, o + l.positions,
+                   reinterpret_cast<int4*>(o + l.plan_q), reinterpret_cast<int4*>(o + l.plan_k)};
   gfs_host::launch_pdl(attention_mask_kernel, dim3(B), dim3(MASK_THREADS), 0, static_cast<cudaStream_t>(stream), a);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
+}
+
+// offsets[9]: where the buffer of a mask has first, last, qfirst, qlast, plan_q, plan_k, padded and positions, and its length.
+void gfs_attention_mask_layout(int B, int S, long long* offsets) {
+  const MaskLayout l = mask_layout(B, S);
+  const size_t at[9] = {l.first, l.last, l.qfirst, l.qlast, l.plan_q, l.plan_k, l.padded, l.positions, l.end};
+  for (int i = 0; i < 9; ++i) offsets[i] = static_cast<long long>(at[i]);
 }
 
 // q [B, nh, S, D], k and v [B, nkv, S, D], out like q; strides: 12 element strides {q, k, v, out} x {seq, batch, head}.
@@ -477,9 +512,7 @@ int gfs_masked_attention_fwd(const void* q, const void* k, const void* v, void* 
   p.score.sl2 = cap > 0.f ? 2.f * scale * LOG2E_F / cap : scale * LOG2E_F;
   p.score.cap2 = cap * LOG2E_F;
   p.score.slopes = static_cast<const float*>(slopes);
-  const int* m = static_cast<const int*>(mask);
-  const size_t n = static_cast<size_t>(B) * S_pad;
-  p.mask = MaskView{m, m + n, m + 2 * n, m + 3 * n, m + 4 * n};
+  p.mask = mask_view(mask, B, S);
   p.status = gfs_host::status_words();
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   return D == 64 ? launch_fwd_scores<64>(tq, tk, tv, p, cap > 0.f, stream)

@@ -16,8 +16,43 @@ namespace gfs {
 struct MaskView {
   const int *first, *last;     // [B, S_pad]: the keys that a query sees
   const int *qfirst, *qlast;   // [B, S_pad]: the queries that see a key
+  const int4 *plan_q, *plan_k; // [B, S_pad / 128]: the tiles of 128 queries (keys), those that see (are seen by) most first
   const int* padded;           // [B]: the sequence has padding
 };
+// An entry of a plan: the tile, the first row that any of its rows sees (for keys: is seen by), one past the last.
+struct TilePlan {
+  int tile, lo, hi;
+};
+__device__ __forceinline__ TilePlan load_plan(const int4* p) {
+  const int4 e = *p;
+  return TilePlan{e.x, e.y, e.z};
+}
+
+// The parts of the buffer that gfs_attention_mask fills: int32 offsets.
+struct MaskLayout {
+  size_t first, last, qfirst, qlast, plan_q, plan_k, padded, positions, end;
+};
+__host__ __device__ inline MaskLayout mask_layout(int B, int S) {
+  const size_t S_pad = (static_cast<size_t>(S) + 127) / 128 * 128;
+  const size_t n = B * S_pad, plan = B * (S_pad / 128) * 4;
+  MaskLayout l;
+  l.first = 0;
+  l.last = n;
+  l.qfirst = 2 * n;
+  l.qlast = 3 * n;
+  l.plan_q = 4 * n;
+  l.plan_k = l.plan_q + plan;
+  l.positions = l.plan_k + plan;
+  l.padded = l.positions + static_cast<size_t>(B) * S;
+  l.end = l.padded + B;
+  return l;
+}
+inline MaskView mask_view(const void* buffer, int B, int S) {
+  const int* m = static_cast<const int*>(buffer);
+  const MaskLayout l = mask_layout(B, S);
+  return MaskView{m + l.first, m + l.last, m + l.qfirst, m + l.qlast, reinterpret_cast<const int4*>(m + l.plan_q),
+                  reinterpret_cast<const int4*>(m + l.plan_k), m + l.padded};
+}
 
 // The softmax's exponents are base 2: score = log2(e) (scale q k, or cap tanh(scale q k / cap)) - slope log2(e) |i - j|.
 struct ScoreArgs {

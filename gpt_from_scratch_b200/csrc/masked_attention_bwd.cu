@@ -83,6 +83,8 @@ masked_dvec_kernel(const __nv_bfloat16* dO, const __nv_bfloat16* O, float* __res
 struct MaskedBwdParams {
   __nv_bfloat16* out1;  // mode 0: dK, mode 1: dQ
   __nv_bfloat16* out2;  // mode 0: dV
+  float* partial;       // mode 0, parts > 1: fp32 [parts][dK, dV][B, nkv, S_pad, D]
+  int parts;            // the heads of a group are dealt to this many items
   long long o1_ss, o1_bs, o1_hs;
   long long o2_ss, o2_bs, o2_hs;
   const float* lse;   // [B, nh, S_pad], base 2
@@ -156,27 +158,55 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     return;
   }
   const int heads = MODE == 0 ? p.nh / p.group : p.nh;
-  const int BH = p.B * heads;
+  const int BHP = p.B * heads * p.parts;
   // the rows that a resident row sees: queries of a key, keys of a query
   const int* const lo_all = MODE == 0 ? p.mask.qfirst : p.mask.first;
   const int* const hi_all = MODE == 0 ? p.mask.qlast : p.mask.last;
-  // Persistent: a CTA walks work items (resident tile, batch * head) dealt in a snake over the CTAs; barrier phases
-  // run on counters that continue across items, so the next item's loads and first score MMAs overlap this one's epilogue.
+  // Persistent: a CTA walks work items (resident tile, batch * head * part), the heaviest first, dealt in a snake over the
+  // CTAs; barrier phases run on counters that continue across items, so the next item's loads and first score MMAs overlap
+  // this one's epilogue.
   const int G = static_cast<int>(gridDim.x);
-  auto snake = [&](int rnd) {
-    return rnd * G + ((rnd & 1) ? G - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
+  const int hpi = MODE == 0 ? p.group / p.parts : 1;    // heads per item
+  const int4* const plans = MODE == 0 ? p.mask.plan_k : p.mask.plan_q;
+  struct Item {
+    int rt, b, h, part, t_begin, n_t;    // n_t: streamed tiles per head (at least one, which may be masked whole)
   };
-  // resident tile, batch and head of work item w, its first streamed tile and their number per head (at least one, which
-  // may be masked whole)
-  auto decode = [&](int w, int& rt, int& b, int& h, int& t_begin, int& n_t) {
-    const int level = w / BH;
-    const int bh = w % BH;
-    rt = MODE == 0 ? level : n_rt - 1 - level;   // under a causal mask the heaviest come first
-    b = bh / heads;
-    h = bh % heads;
-    const size_t row = static_cast<size_t>(b) * p.S_pad;
-    t_begin = lo_all[row + rt * 128] >> 6;
-    n_t = max(((hi_all[row + min(rt * 128 + 127, p.S - 1)] + 63) >> 6) - t_begin, 1);
+  struct Walk {                          // the items of this CTA, the next one's plan already on its way
+    int it, w;
+    int4 plan;
+  };
+  auto where = [&](int it) { return it * G + ((it & 1) ? G - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x)); };
+  auto split = [&](int w, int& b, int& h, int& part) {
+    int r = w % BHP;
+    part = r % p.parts;
+    r /= p.parts;
+    h = r % heads;
+    b = r / heads;
+  };
+  auto fetch = [&](Walk& k) {
+    k.w = where(k.it);
+    if (k.w < n_items) {
+      int b, h, part;
+      split(k.w, b, h, part);
+      k.plan = plans[static_cast<size_t>(b) * n_rt + k.w / BHP];
+    }
+  };
+  auto start = [&]() {
+    Walk k;
+    k.it = 0;
+    fetch(k);
+    return k;
+  };
+  // the next item, or false: an item past the end can only occur in a CTA's last round
+  auto next = [&](Walk& k, Item& i) {
+    if (k.w >= n_items) return false;
+    split(k.w, i.b, i.h, i.part);
+    i.rt = k.plan.x;
+    i.t_begin = k.plan.y >> 6;
+    i.n_t = max(((k.plan.z + 63) >> 6) - i.t_begin, 1);
+    ++k.it;
+    fetch(k);
+    return true;
   };
 
   if (threadIdx.x == 0) {
@@ -219,11 +249,10 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
   if (warp == 0) {
     if (lane == 0) {
       int g = 0;  // streamed tiles loaded so far (ring position)
-      for (int it = 0; it * G < n_items; ++it) {
-        const int w = snake(it);
-        if (w >= n_items) break;
-        int rt, b, h, t_begin, n_t;
-        decode(w, rt, b, h, t_begin, n_t);
+      Walk walk = start();
+      Item item;
+      for (int it = 0; next(walk, item); ++it) {
+        const int rt = item.rt, b = item.b, h = item.h, t_begin = item.t_begin, n_t = item.n_t;
         mbar_wait(r_empty, (it & 1) ^ 1u, wctx, STATUS_TIMEOUT_PIPE_EMPTY);  // previous item's score MMAs done
         mbar_arrive_expect_tx(r_full, 2 * R_BYTES);
 #pragma unroll
@@ -231,9 +260,8 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
           tma_load_4d(R1 + db * 16384, &tr1, r_full, db * 64, rt * 128, h, b);
           tma_load_4d(R2 + db * 16384, &tr2, r_full, db * 64, rt * 128, h, b);
         }
-        const int n_heads = MODE == 0 ? p.group : 1;
-        for (int hh = 0; hh < n_heads; ++hh) {
-          const int th = MODE == 0 ? h * p.group + hh : h / p.group;   // head of the streamed tiles
+        for (int hh = 0; hh < hpi; ++hh) {
+          const int th = MODE == 0 ? h * p.group + item.part * hpi + hh : h / p.group;   // head of the streamed tiles
           for (int t = 0; t < n_t; ++t, ++g) {
             const int st = g % TS;
             const int ti = t_begin + t;
@@ -260,13 +288,12 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     constexpr uint32_t idesc_xy = umma_idesc_bf16(128, 64, 0, 0);
     const uint32_t r1 = smem_u32(R1), r2 = smem_u32(R2);
     int g = 0;
-    for (int it = 0; it * G < n_items; ++it) {
-      const int w = snake(it);
-      if (w >= n_items) break;
-      int rt, b, h, t_begin, n_t;
-      decode(w, rt, b, h, t_begin, n_t);
+    Walk walk = start();
+    Item item;
+    for (int it = 0; next(walk, item); ++it) {
+      const int b = item.b, t_begin = item.t_begin, n_t = item.n_t;
       const bool padded = p.mask.padded[b] != 0;
-      const int n = MODE == 0 ? n_t * p.group : n_t;
+      const int n = n_t * hpi;
       mbar_wait(r_full, it & 1, wctx, STATUS_TIMEOUT_PIPE_FULL);
       for (int t = 0; t < n; ++t, ++g) {
         const int st = g % TS, sb = g & 1;
@@ -288,12 +315,10 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     // gradient MMAs
     constexpr uint32_t idesc_acc = umma_idesc_bf16(128, D, 0, 1);
     int g = 0;
-    for (int it = 0; it * G < n_items; ++it) {
-      const int w = snake(it);
-      if (w >= n_items) break;
-      int rt, b, h, t_begin, n_t;
-      decode(w, rt, b, h, t_begin, n_t);
-      const int n = MODE == 0 ? n_t * p.group : n_t;
+    Walk walk = start();
+    Item item;
+    for (int it = 0; next(walk, item); ++it) {
+      const int n = item.n_t * hpi;
       for (int t = 0; t < n; ++t, ++g) {
         const int st = g % TS, sb = g & 1;
         mbar_wait(&m_full[sb], (g >> 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
@@ -329,12 +354,12 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     uint8_t* stage = staging + cw * Shape::STAGE_BYTES;
     bool acc_pending = false;           // the previous item's acc_full phase has not been waited for
     int g0 = 0;
-    for (int it = 0; it * G < n_items; ++it) {
-      const int w = snake(it);
-      if (w >= n_items) break;
-      int rt, b, h, t_begin, n_t;
-      decode(w, rt, b, h, t_begin, n_t);
-      const int n = MODE == 0 ? n_t * p.group : n_t;
+    Walk walk = start();
+    Item item;
+    for (int it = 0; next(walk, item); ++it) {
+      const int rt = item.rt, b = item.b, h = item.h, t_begin = item.t_begin, n_t = item.n_t;
+      const int head0 = MODE == 0 ? h * p.group + item.part * hpi : h;   // query head of the item's first tiles
+      const int n = n_t * hpi;
       const int row_g = rt * 128 + r;  // mode 0: key position, mode 1: query position
       const int* lo_b = lo_all + static_cast<size_t>(b) * p.S_pad;
       const int* hi_b = hi_all + static_cast<size_t>(b) * p.S_pad;
@@ -376,7 +401,7 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
             __syncwarp();
             if (lane == 0) mbar_arrive(&xy_empty[group]);
           }
-          const float slope2 = DIST ? p.score.slopes[MODE == 0 ? h * p.group + hh : h] * LOG2E_F : 0.f;
+          const float slope2 = DIST ? p.score.slopes[head0 + hh] * LOG2E_F : 0.f;
           const float dist0 = static_cast<float>(row_g - col0);
           const int a = lo - col0;
           const unsigned width = static_cast<unsigned>(hi - lo);
@@ -490,10 +515,23 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
           __syncwarp();
           if (lane == 0) mbar_arrive(acc_empty);
         }
+        if (MODE == 0 && p.parts > 1) {
+          // fp32, one part of the sum: 16 columns at a time, the width of a staged row
+          float* to = p.partial + (((static_cast<size_t>(item.part) * 2 + is_dv) * p.B + b) * heads + h) * p.S_pad * D +
+                      static_cast<size_t>(row0) * D + c;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          wv[e] = seen ? pack_bf16x2(__uint_as_float(v[2 * e]) * out_scale, __uint_as_float(v[2 * e + 1]) * out_scale) : 0u;
-        store_rows_32x32(stage, wv, lane, out + c, o_ss, p.S - row0);
+          for (int c2 = 0; c2 < 2; ++c2) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              wv[e] = seen ? __float_as_uint(__uint_as_float(v[16 * c2 + e]) * out_scale) : 0u;
+            store_rows_32x32(stage, wv, lane, reinterpret_cast<__nv_bfloat16*>(to + 16 * c2), 2 * D, p.S - row0);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            wv[e] = seen ? pack_bf16x2(__uint_as_float(v[2 * e]) * out_scale, __uint_as_float(v[2 * e + 1]) * out_scale) : 0u;
+          store_rows_32x32(stage, wv, lane, out + c, o_ss, p.S - row0);
+        }
       }
     }
   }
@@ -505,6 +543,43 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
   if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
 }
 
+// dK and dV from the parts' sums, added in their order. D / 8 threads per row of [B, nkv, S].
+__global__ void __launch_bounds__(256)
+masked_dkv_kernel(const float* partial, int parts, __nv_bfloat16* __restrict__ dk, __nv_bfloat16* __restrict__ dv, int S,
+                  int S_pad, int B, int nkv, int D, long long k_ss, long long k_bs, long long k_hs, long long v_ss,
+                  long long v_bs, long long v_hs) {
+  pdl_wait();
+  pdl_trigger();
+  const int tpr = D >> 3;
+  const size_t n = static_cast<size_t>(B) * nkv * S_pad * D;     // elements of one tensor of one part
+  const unsigned total = 2u * B * nkv * S;
+  for (unsigned row = blockIdx.x * (256 / tpr) + threadIdx.x / tpr; row < total; row += gridDim.x * (256 / tpr)) {
+    const int c = (threadIdx.x % tpr) * 8;
+    const unsigned is_dv = row >= total / 2;
+    const unsigned r = row - is_dv * (total / 2);
+    const unsigned s = r % S, bh = r / S;
+    const float* from = partial + is_dv * n + (static_cast<size_t>(bh) * S_pad + s) * D + c;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), z = a;
+    for (int i = 0; i < parts; ++i) {
+      const float4 x = *reinterpret_cast<const float4*>(from + 2 * n * i), y = *reinterpret_cast<const float4*>(from + 2 * n * i + 4);
+      a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+      z.x += y.x; z.y += y.y; z.z += y.z; z.w += y.w;
+    }
+    const unsigned b = bh / nkv, h = bh % nkv;
+    __nv_bfloat16* to = is_dv ? dv + s * v_ss + b * v_bs + h * v_hs : dk + s * k_ss + b * k_bs + h * k_hs;
+    *reinterpret_cast<uint4*>(to + c) = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(z.x, z.y),
+                                                   pack_bf16x2(z.z, z.w));
+  }
+}
+
+// Into how many parts the heads of a group are dealt for dK and dV.
+int group_parts(int tiles, int B, int nkv, int group) {
+  int parts = 1;
+  while (parts < 4 && group % (2 * parts) == 0 && static_cast<long long>(tiles) * B * nkv * parts < 4ll * gfs_host::sm_count())
+    parts *= 2;
+  return tiles > 1 ? parts : 1;
+}
+
 struct BwdMaps {
   const CUtensorMap *q128, *k128, *v128, *do128, *q64, *k64, *v64, *do64;
 };
@@ -513,7 +588,7 @@ template <int D, bool CAP, bool DIST>
 int launch_bwd(const BwdMaps& m, const MaskedBwdParams& p0, const MaskedBwdParams& p1, cudaStream_t stream) {
   static gfs_host::SmemLimit limit0, limit1;
   const int n_rt = p0.S_pad / 128;
-  const int items0 = n_rt * p0.B * (p0.nh / p0.group), items1 = n_rt * p0.B * p0.nh;
+  const int items0 = n_rt * p0.B * (p0.nh / p0.group) * p0.parts, items1 = n_rt * p0.B * p0.nh;
   constexpr int smem0 = MBwdShape<D, 0>::SMEM, smem1 = MBwdShape<D, 1>::SMEM;
   if (!limit0.raise(masked_bwd_kernel<D, 0, CAP, DIST>, smem0) || !limit1.raise(masked_bwd_kernel<D, 1, CAP, DIST>, smem1))
     return -10;
@@ -535,11 +610,20 @@ int launch_bwd_scores(const BwdMaps& m, const MaskedBwdParams& p0, const MaskedB
 
 extern "C" {
 
+// fp32 elements of the scratch `partial` of the backward (0: none)
+long long gfs_masked_attention_scratch(int S, int B, int nh, int nkv, int D) {
+  const int tiles = (S + 127) / 128;
+  const int parts = group_parts(tiles, B, nkv, nh / nkv);
+  return parts > 1 ? 2ll * parts * B * nkv * tiles * 128 * D : 0;
+}
+
 // strides: 24 element strides for {q, k, v, out, dout, dq, dk, dv} x {seq, batch, head}; lse (from the forward) and dvec
-// (scratch): fp32 [B, nh, S_pad]; the rest as for gfs_masked_attention_fwd. dq shares no memory with anything that is read
+// (scratch): fp32 [B, nh, S_pad]; partial: scratch of the
+// size above; the rest as for gfs_masked_attention_fwd. dq shares no memory with anything that is read
 // for dk and dv, nor with them: its kernel runs beside theirs.
 int gfs_masked_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout,
-                             const void* lse, void* dvec, void* dq, void* dk, void* dv, const void* mask, int S, int B,
+                             const void* lse, void* dvec, void* partial, void* dq, void* dk, void* dv,
+                             const void* mask, int S, int B,
                              int nh, int nkv, int D, const long long* strides, float scale, float cap, const void* slopes,
                              void* stream_) {
   if ((D != 64 && D != 128) || !strides_ok(strides, 24) || nkv <= 0 || nh % nkv != 0) return -1;
@@ -553,10 +637,8 @@ int gfs_masked_attention_bwd(const void* q, const void* k, const void* v, const 
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const long long *sq = strides, *sk = strides + 3, *sv = strides + 6, *so = strides + 9, *sdo = strides + 12,
                   *sdq = strides + 15, *sdk = strides + 18, *sdv = strides + 21;
-  const int* m = static_cast<const int*>(mask);
-  const size_t n = static_cast<size_t>(B) * S_pad;
   MaskedBwdParams p = {};
-  p.mask = MaskView{m, m + n, m + 2 * n, m + 3 * n, m + 4 * n};
+  p.mask = mask_view(mask, B, S);
   {
     const long long rows = static_cast<long long>(S_pad) * B * nh;
     const int threads = 256;
@@ -579,12 +661,23 @@ int gfs_masked_attention_bwd(const void* q, const void* k, const void* v, const 
   p.score.cap2 = cap * LOG2E_F;
   p.score.slopes = static_cast<const float*>(slopes);
   p.status = gfs_host::status_words();
+  p.parts = 1;
   MaskedBwdParams p0 = p, p1 = p;
+  p0.parts = group_parts(S_pad / 128, B, nkv, nh / nkv);
+  p0.partial = static_cast<float*>(partial);
   p0.out1 = static_cast<__nv_bfloat16*>(dk); p0.o1_ss = sdk[0]; p0.o1_bs = sdk[1]; p0.o1_hs = sdk[2];
   p0.out2 = static_cast<__nv_bfloat16*>(dv); p0.o2_ss = sdv[0]; p0.o2_bs = sdv[1]; p0.o2_hs = sdv[2];
   p1.out1 = static_cast<__nv_bfloat16*>(dq); p1.o1_ss = sdq[0]; p1.o1_bs = sdq[1]; p1.o1_hs = sdq[2];
-  return D == 64 ? launch_bwd_scores<64>(maps, p0, p1, cap > 0.f, stream)
-                 : launch_bwd_scores<128>(maps, p0, p1, cap > 0.f, stream);
+  const int rc = D == 64 ? launch_bwd_scores<64>(maps, p0, p1, cap > 0.f, stream)
+                         : launch_bwd_scores<128>(maps, p0, p1, cap > 0.f, stream);
+  if (rc != 0 || p0.parts == 1) return rc;
+  const long long rows = 2ll * B * nkv * S;
+  const int rows_per_block = 256 / (D >> 3);
+  const dim3 grid(static_cast<unsigned>(std::min<long long>((rows + rows_per_block - 1) / rows_per_block, gfs_host::sm_count() * 32)));
+  gfs_host::launch_pdl(masked_dkv_kernel, grid, dim3(256), 0, stream, static_cast<const float*>(partial), p0.parts,
+                       static_cast<__nv_bfloat16*>(dk), static_cast<__nv_bfloat16*>(dv), S, S_pad, B, nkv, D, sdk[0], sdk[1],
+                       sdk[2], sdv[0], sdv[1], sdv[2]);
+  return cudaGetLastError() == cudaSuccess ? 0 : -14;
 }
 
 }  // extern "C"

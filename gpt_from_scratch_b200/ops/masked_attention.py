@@ -31,10 +31,10 @@ class AttentionMask:
         if self._parts is not None:
             return self._parts[i]
         B, S = self.batch, self.seq_len
-        S_pad = _pad128(S)
+        layout = _layout(B, S)
         if i == 2:
-            return self.buffer.as_strided((B, S), (S, 1), 4 * B * S_pad + B)
-        return self.buffer.as_strided((B, S), (S_pad, 1), i * B * S_pad)
+            return self.buffer.as_strided((B, S), (S, 1), layout["positions"])
+        return self.buffer.as_strided((B, S), (_pad128(S), 1), layout["last" if i else "first"])
 
     @property
     def first(self) -> torch.Tensor:
@@ -52,6 +52,14 @@ class AttentionMask:
         """bool ``[B, S, S]``, query by key."""
         at = torch.arange(self.seq_len, device=self.device)
         return (at >= self.first.unsqueeze(-1)) & (at < self.last.unsqueeze(-1))
+
+
+@functools.lru_cache(maxsize=256)
+def _layout(B: int, S: int) -> dict[str, int]:
+    """Where a mask's buffer has its parts, and its length."""
+    at = (ctypes.c_longlong * 9)()
+    _lib.lib().gfs_attention_mask_layout(B, S, at)
+    return dict(zip(("first", "last", "qfirst", "qlast", "plan_q", "plan_k", "padded", "positions", "end"), at))
 
 
 def _pad128(S: int) -> int:
@@ -113,7 +121,7 @@ def attention_mask(batch: int, seq_len: int, causal: bool = True, document_ids: 
     ids = None if document_ids is None else document_ids.contiguous()
     prefix = None if prefix_mask is None else prefix_mask.contiguous()
     B, S = batch, seq_len
-    buffer = torch.empty(4 * B * _pad128(S) + B + B * S, dtype=torch.int32, device=device)
+    buffer = torch.empty(_layout(B, S)["end"], dtype=torch.int32, device=device)
     with _lib.on_device(buffer), _lib.nvtx("attention_mask"):
         rc = _lib.lib().gfs_attention_mask(_lib.ptr(ids), ids is not None and ids.dtype == torch.int64, _lib.ptr(prefix), B,
                                            S, causal, min(window or 0, 0x7fffffff), buffer.data_ptr(), _lib.stream_ptr())
@@ -180,6 +188,11 @@ def _forward(q, k, v, buffer, slopes, softcap: float, scale: float, want_lse: bo
     return out, lse
 
 
+@functools.lru_cache(maxsize=256)
+def _scratch(S: int, B: int, nh: int, nkv: int, D: int) -> int:
+    return _lib.lib().gfs_masked_attention_scratch(S, B, nh, nkv, D)
+
+
 class _MaskedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, buffer, slopes, softcap, scale):
@@ -201,15 +214,17 @@ class _MaskedAttention(torch.autograd.Function):
         kv = k.shape
         dout = _readable(dout)
         dvec = torch.empty_like(lse)
+        scratch = _scratch(S, B, nh, kv[1], D)
+        partial = torch.empty(scratch, dtype=torch.float32, device=q.device) if scratch else None
         st = _stride_array(shape, q.stride(), kv, k.stride(), kv, v.stride(), shape, out.stride(), shape, dout.stride(), shape,
                            dq.stride(), kv, dk.stride(), kv, dv.stride())
         with _lib.on_device(q), _lib.nvtx("masked_attention_bwd"):
             rc = _lib.lib().gfs_masked_attention_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                                     dout.data_ptr(), lse.data_ptr(), dvec.data_ptr(), dq.data_ptr(),
-                                                     dk.data_ptr(), dv.data_ptr(), buffer.data_ptr(), S, B, nh, kv[1], D,
-                                                     st, scale, softcap, _lib.ptr(slopes), _lib.stream_ptr())
+                                                     dout.data_ptr(), lse.data_ptr(), dvec.data_ptr(), _lib.ptr(partial),
+                                                     dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), buffer.data_ptr(), S, B,
+                                                     nh, kv[1], D, st, scale, softcap, _lib.ptr(slopes), _lib.stream_ptr())
         _lib.check(rc, "gfs_masked_attention_bwd")
-        _lib.add_launches(2)  # pre-pass + two main kernels
+        _lib.add_launches(3 if scratch else 2)  # pre-pass + two main kernels (+ the sum of the parts)
         return dq, dk, dv, None, None, None, None
 
 

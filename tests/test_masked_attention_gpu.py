@@ -19,6 +19,7 @@ import torch
 
 from gpt_from_scratch_b200 import ops
 from gpt_from_scratch_b200.ops import _lib
+from gpt_from_scratch_b200.ops.masked_attention import _layout, _scratch
 
 pytestmark = pytest.mark.gpu
 U, F = 2.0 ** -8, 2.0 ** -12
@@ -110,8 +111,13 @@ def test_mask(cuda_device, B, S, kind):
                 assert torch.equal(getattr(mask, name).cpu(), getattr(cpu, name)), f"{name} {causal} {window}"
         # the queries of every key, as the backward reads them
         S_pad = (S + 127) // 128 * 128
-        n = B * S_pad
-        qfirst, qlast = (mask.buffer[i * n:(i + 1) * n].view(B, S_pad).cpu() for i in (2, 3))
+        tiles = S_pad // 128
+        layout = _layout(B, S)
+        assert mask.buffer.numel() == layout["end"]
+        qfirst, qlast, padded, plan_q, plan_k = (
+            mask.buffer[layout[name]:layout[name] + math.prod(shape)].view(shape).cpu()
+            for name, shape in (("qfirst", (B, S_pad)), ("qlast", (B, S_pad)), ("padded", (B,)), ("plan_q", (B, tiles, 4)),
+                                ("plan_k", (B, tiles, 4))))
         see = cpu.visible()
         j_any = see.any(1)
         rows = torch.arange(S)[None, :, None]
@@ -121,8 +127,15 @@ def test_mask(cuda_device, B, S, kind):
         assert torch.equal(torch.where(j_any, qlast[:, :S], 0), torch.where(j_any, hi, 0).int())
         assert (qfirst[:, :S][~j_any] == qlast[:, :S][~j_any]).all() and (qfirst[:, S:] == S).all() and (qlast[:, S:] == S).all()
         assert (qfirst.diff(dim=1) >= 0).all() and (qlast.diff(dim=1) >= 0).all()
-        assert mask.buffer[4 * n:4 * n + B].cpu().bool().tolist() == [False] * B if ids is None else \
-            mask.buffer[4 * n:4 * n + B].cpu().bool().tolist() == (ids < 0).any(1).tolist()
+        assert padded.bool().tolist() == ([False] * B if ids is None else (ids < 0).any(1).tolist())
+        # the order of the tiles: every one once, with the ends of what it sees, the widest first
+        ends = torch.arange(tiles) * 128, (torch.arange(tiles) * 128 + 127).clamp_max(S - 1)
+        for plan, lo, hi in ((plan_q, cpu.first, cpu.last), (plan_k, qfirst, qlast)):
+            for b in range(B):
+                t = plan[b, :, 0].long()
+                assert t.sort().values.tolist() == list(range(tiles))
+                assert torch.equal(plan[b, :, 1], lo[b][ends[0][t]]) and torch.equal(plan[b, :, 2], hi[b][ends[1][t]])
+                assert ((plan[b, :, 2] - plan[b, :, 1]).diff() <= 0).all()
 
 
 #   B, nh, nkv, S, D, documents, causal, prefix, window, cap, distance
@@ -180,7 +193,7 @@ def test_masked_attention(cuda_device, form):
         want, tols = bounds_and_values(q, k, v, do, mask.visible(), cap, slopes, 1 / math.sqrt(D))
         check([out], want, tols, "forward")
         got = run(q, k, v, do, mask, softcap=cap, alibi_slopes=slopes)
-        assert _lib.launch_count() - before == 5
+        assert _lib.launch_count() - before == 5 + (_scratch(S, B, nh, nkv, D) > 0)
         check(got, want, tols, f"packed {packed}")
         assert torch.equal(got[0], out)
         hidden = ~mask.visible().any(2)[:, None, :, None]
