@@ -57,18 +57,20 @@ struct MaskArgs {
   const uint8_t* prefix;    // [B, S] or null
   int ids64, S, S_pad, window, causal;
   int *first, *last, *qfirst, *qlast, *padded, *positions;
-  int4 *plan_q, *plan_k;
+  int4 *plan_q, *plan_k, *pairs;
 };
 
 // The tiles of a sequence in descending order of the rows between their ends (the work they are): kernels that start the
 // heaviest first end together. Ranks by counting; a longer sequence than fits has enough tiles to even out by itself.
 constexpr int MASK_SORT = 2048;
-__device__ __forceinline__ void sort_tiles(const int* lo, const int* hi, int S, int4* plan, int* weight) {
-  const int n = (S + 127) >> 7;
+// ROWS: of a tile. `put` writes the entry of a tile at its rank.
+template <int ROWS, typename Put>
+__device__ __forceinline__ void sort_tiles(const int* lo, const int* hi, int S, int* weight, Put put) {
+  const int n = (S + ROWS - 1) / ROWS;
   const bool sorted = n <= MASK_SORT;
   __syncthreads();
   for (int t = threadIdx.x; t < n; t += MASK_THREADS)
-    if (sorted) weight[t] = hi[min(t * 128 + 127, S - 1)] - lo[t * 128];
+    if (sorted) weight[t] = hi[min((t + 1) * ROWS, S) - 1] - lo[t * ROWS];
   __syncthreads();
   for (int t = threadIdx.x; t < n; t += MASK_THREADS) {
     int rank = n - 1 - t;
@@ -77,7 +79,7 @@ __device__ __forceinline__ void sort_tiles(const int* lo, const int* hi, int S, 
       const int mine = weight[t];
       for (int u = 0; u < n; ++u) rank += weight[u] > mine || (weight[u] == mine && u > t);
     }
-    plan[rank] = make_int4(t, lo[t * 128], hi[min(t * 128 + 127, S - 1)], 0);
+    put(rank, t);
   }
 }
 
@@ -131,7 +133,7 @@ __global__ void __launch_bounds__(MASK_THREADS) attention_mask_kernel(const Mask
         qlast = min(qlast, i + a.window);
       }
       if (id_of(i) < 0) {
-        first = last = qfirst = qlast = start;
+        first = last = qfirst = qlast = i;      // wherever it does not widen a tile's range
         any = 1;
       }
       a.first[prow + i] = first;
@@ -146,57 +148,90 @@ __global__ void __launch_bounds__(MASK_THREADS) attention_mask_kernel(const Mask
   any = __syncthreads_or(any);
   if (threadIdx.x == 0) a.padded[b] = any;
   const size_t tiles = static_cast<size_t>(b) * (a.S_pad / 128);
-  sort_tiles(a.first + prow, a.last + prow, a.S, a.plan_q + tiles, weight);
-  sort_tiles(a.qfirst + prow, a.qlast + prow, a.S, a.plan_k + tiles, weight);
+  const int *first = a.first + prow, *last = a.last + prow, *qfirst = a.qfirst + prow, *qlast = a.qlast + prow;
+  auto end = [&](const int* hi, int t) { return hi[min(t * 128 + 127, a.S - 1)]; };
+  sort_tiles<128>(first, last, a.S, weight, [&](int rank, int t) {
+    a.plan_q[tiles + rank] = make_int4(t, first[t * 128], end(last, t), any);
+  });
+  sort_tiles<128>(qfirst, qlast, a.S, weight, [&](int rank, int t) {
+    a.plan_k[tiles + rank] = make_int4(t, qfirst[t * 128], end(qlast, t), any);
+  });
+  int4* const pairs = a.pairs + static_cast<size_t>(b) * ((a.S_pad / 128 + 1) / 2) * 2;
+  sort_tiles<256>(first, last, a.S, weight, [&](int rank, int t) {
+    const bool two = t * 256 + 128 < a.S;
+    const int la = first[t * 256], ha = end(last, 2 * t);
+    const int lb = two ? first[t * 256 + 128] : 0, hb = two ? end(last, 2 * t + 1) : 0;
+    int a0 = la >> 6, a1 = (ha + 63) >> 6, b0 = lb >> 6, b1 = (hb + 63) >> 6;
+    if (a1 <= a0) {               // all padding: one block, of the other tile's
+      a0 = two && b1 > b0 ? b0 : a0;
+      a1 = a0 + 1;
+    }
+    if (two && b1 <= b0) {
+      b0 = a1 - 1;
+      b1 = a1;
+    }
+    pairs[2 * rank] = make_int4(t, a0, a1, b0);
+    pairs[2 * rank + 1] = make_int4(b1, any, 0, 0);
+  });
 }
 
 // ---------------------------------------------------------------------------
-// Forward. A CTA has one tile of 128 queries of a head: TMA warp, MMA warp, eight softmax warps and half of the tensor memory (S | O),
-// so two CTAs share an SM and each fills the other's waits. Two warps share the 32 rows of a quarter, 64 of a block's 128
-// keys each, and exchange their row maxima through shared memory; P overwrites the scores that it was made from, in tensor memory.
+// Forward. One persistent CTA per SM walks items of two tiles of 128 queries that share the loads of their keys: two heads of a
+// group at the same queries (groups of an even number), else neighbouring tiles of a head. A thread per query row.
 // ---------------------------------------------------------------------------
 struct MaskedFwdParams {
   __nv_bfloat16* O;
   long long o_ss, o_bs, o_hs;  // element strides: sequence, batch, head
-  float* lse;                  // [B, nh, S_pad], base 2; +inf for rows that see nothing
+  float* lse;                  // [B, nh, S_pad], base 2; +inf for rows that see nothing; or null
   int S, S_pad, B, nh, group;
+  int head_pairs;
   ScoreArgs score;
   MaskView mask;
   uint32_t* status;
 };
 
-constexpr int MFWD_CW = 8;
-constexpr int MFWD_THREADS = 32 * (2 + MFWD_CW);
+constexpr int MFWD_FIRST_SW = 4;                    // warps 0: TMA, 1 and 2: the MMAs of a tile, 3: idle; then the softmax warps
+constexpr int MFWD_THREADS = 32 * (MFWD_FIRST_SW + 8);
+// 384 threads x 168 at the launch = 128 x 72 + 256 x 216: a softmax thread holds the 128 scores of its row.
+constexpr int MFWD_REGS_IO = 72, MFWD_REGS_SOFTMAX = 216;
 template <int D>
 struct MFwdShape {
   static constexpr int DB = D / 64;
-  static constexpr int TILE = DB * 16384;
-  static constexpr int KS = D == 64 ? 2 : 1;      // stages of K and V
-  static constexpr int SMEM = TILE * (1 + 2 * KS) + 2048 + 256;
+  static constexpr int Q_TILE = DB * 16384, KV_TILE = DB * 8192;    // 128 queries, 64 keys
+  static constexpr int KS = D == 64 ? 8 : 4;        // stages of K and V
+  static constexpr int STAGING = 8 * 4096;          // to transpose the output rows through
+  static constexpr int SMEM = 2 * Q_TILE + 2 * KS * KV_TILE + STAGING + 512;
 };
+// Scores: as they are, capped with a bound that the running maximum may be left out for, capped.
+enum Scores { PLAIN = 0, BOUNDED = 1, CAPPED = 2 };
+// Up to this cap2 no maximum is needed: probabilities lie within 2^-80 and 2^80, which leaves fp32 sums (and bf16, which has the
+// same exponents) a factor of 2^46 on either side.
+constexpr float BOUNDED_CAP2 = 80.f;
 
-template <int D, bool CAP, bool DIST>
-__global__ void __launch_bounds__(MFWD_THREADS, 2)
+template <int D, int SCORES, bool DIST>
+__global__ void __launch_bounds__(MFWD_THREADS, 1)
 masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                  const __grid_constant__ CUtensorMap tv, const MaskedFwdParams p, int n_tiles) {
+                  const __grid_constant__ CUtensorMap tv, const MaskedFwdParams p, int n_levels, int n_items) {
   using Shape = MFwdShape<D>;
-  constexpr int DB = Shape::DB, TILE = Shape::TILE, KS = Shape::KS;
-  constexpr uint32_t O_COL = 128, P_HALF = 64;
+  constexpr int DB = Shape::DB, Q_TILE = Shape::Q_TILE, KV_TILE = Shape::KV_TILE, KS = Shape::KS;
+  constexpr uint32_t O_COL = 256;            // scores at [tile][buffer][64] before that; P takes the columns of its scores
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* Qs = smem_raw;
-  uint8_t* Ks = Qs + TILE;
-  uint8_t* Vs = Ks + KS * TILE;
-  float* xch = reinterpret_cast<float*>(Vs + KS * TILE);     // [parity][half][row]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(xch + 512);
+  uint8_t* Qs = smem_raw;                    // [2] tiles
+  uint8_t* Ks = Qs + 2 * Q_TILE;             // [KS]
+  uint8_t* Vs = Ks + KS * KV_TILE;           // [KS]
+  uint8_t* staging = Vs + KS * KV_TILE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + Shape::STAGING);
   uint64_t* q_full = bars;
-  uint64_t* s_full = bars + 1;
-  uint64_t* o_full = bars + 2;
-  uint64_t* p_full = bars + 3;
-  uint64_t* k_full = bars + 4;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* k_full = bars + 2;               // [KS]
   uint64_t* k_empty = k_full + KS;
   uint64_t* v_full = k_empty + KS;
   uint64_t* v_empty = v_full + KS;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + KS);
+  uint64_t* s_full = v_empty + KS;           // [tile][buffer]
+  uint64_t* p_full = s_full + 4;
+  uint64_t* o_full = p_full + 4;             // P V of the buffer is done
+  uint64_t* o_empty = o_full + 4;            // [tile]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -206,7 +241,20 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
     return;
   }
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 4 + 4 * KS; ++i) mbar_init(&bars[i], i == 3 ? MFWD_CW : 1);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 2);
+    for (int i = 0; i < KS; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 2);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 2);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    for (int x = 0; x < 2; ++x) mbar_init(&o_empty[x], 4);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tq);
@@ -214,7 +262,7 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
     tma_prefetch_desc(&tv);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 256);
+    tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -225,236 +273,393 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
   const uint32_t tmem_base = *tmem_slot;
   WaitCtx wctx{abort_flag, p.status, GFS_WAIT_LIMIT_NS};
 
-  const int BH = p.B * p.nh;
-  const int level = static_cast<int>(blockIdx.x / BH);                // the tiles that see the most keys come first
-  const int bh = static_cast<int>(blockIdx.x % BH);
-  const int b = bh / p.nh, h = bh % p.nh, kvh = h / p.group;
-  const TilePlan plan = load_plan(p.mask.plan_q + static_cast<size_t>(b) * n_tiles + level);
-  const int* first = p.mask.first + static_cast<size_t>(b) * p.S_pad;
-  const int* last = p.mask.last + static_cast<size_t>(b) * p.S_pad;
-  const int row_a = plan.tile * 128, row_z = min(row_a + 127, p.S - 1);
-  // blocks [j0, j1) of 128 keys; at least one, which may be masked whole
-  const int j0 = plan.lo >> 7;
-  const int j1 = max(j0 + 1, (plan.hi + 127) >> 7);
-
-  if (warp == 0) {
-    if (lane == 0) {
-      auto load = [&](uint8_t* dst, const CUtensorMap& map, uint64_t* full, int row, int head) {
-        mbar_arrive_expect_tx(full, TILE);
-#pragma unroll
-        for (int db = 0; db < DB; ++db) tma_load_4d(dst + db * 16384, &map, full, db * 64, row, head, b);   // rows past S: zeros
-      };
-      load(Qs, tq, q_full, row_a, h);
-      for (int j = j0; j < j1; ++j) {
-        const int g = j - j0, st = g % KS;
-        const uint32_t par = ((g / KS) & 1) ^ 1u;
-        mbar_wait(&k_empty[st], par, wctx, STATUS_TIMEOUT_PIPE_EMPTY);
-        load(Ks + st * TILE, tk, &k_full[st], j * 128, kvh);
-        mbar_wait(&v_empty[st], par, wctx, STATUS_TIMEOUT_PIPE_EMPTY);
-        load(Vs + st * TILE, tv, &v_full[st], j * 128, kvh);
+  // Items: the widest first, dealt to the CTAs in a snake; all barrier parities run on counters that continue across
+  // items. The plan of the next item is on its way while one is worked on.
+  const int heads = p.head_pairs ? p.nh / 2 : p.nh;
+  const int BH = p.B * heads;
+  const int G = static_cast<int>(gridDim.x);
+  struct Item {
+    int b, h[2], row[2];        // batch, heads and first query rows of the two tiles
+    int j0[2], j1[2];           // their blocks of 64 keys; j0 == j1: there is no second tile
+    bool padded;
+  };
+  struct Walk {
+    int it, w;
+    int4 e0, e1;
+  };
+  auto fetch = [&](Walk& k) {
+    k.w = k.it * G + ((k.it & 1) ? G - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
+    if (k.w < n_items) {
+      const size_t at = static_cast<size_t>((k.w % BH) / heads) * n_levels + k.w / BH;
+      if (p.head_pairs) {
+        k.e0 = p.mask.plan_q[at];
+      } else {
+        k.e0 = p.mask.pairs[2 * at];
+        k.e1 = p.mask.pairs[2 * at + 1];
       }
-      settle_copies(wctx);
     }
-  } else if (warp == 1) {
-    // whole warp, converged: the MMA / commit helpers elect the issuing lane
-    constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128, 0, 0);
-    constexpr uint32_t idesc_o = umma_idesc_bf16(128, D, 0, 1);
-    const bool padded = p.mask.padded[b] != 0;
-    mbar_wait(q_full, 0, wctx, STATUS_TIMEOUT_PIPE_FULL);
-    auto issue_s = [&](int j) {
-      const int g = j - j0, st = g % KS;
-      mbar_wait(&k_full[st], (g / KS) & 1, wctx, STATUS_TIMEOUT_PIPE_FULL);
-      if (padded) zero_padding(Ks + st * TILE, 128, DB, 16384, first + j * 128, last + j * 128, lane);
-      tc_fence_after();
-      mma_kk<D / 16>(tmem_base, smem_u32(Qs), 16384, smem_u32(Ks + st * TILE), 16384, idesc_s, false);
-      umma_commit_e(s_full);
-      umma_commit_e(&k_empty[st]);
-    };
-    issue_s(j0);
-    for (int j = j0; j < j1; ++j) {
-      const int g = j - j0, st = g % KS;
-      mbar_wait(&v_full[st], (g / KS) & 1, wctx, STATUS_TIMEOUT_PIPE_FULL);
-      if (padded) zero_padding(Vs + st * TILE, 128, DB, 16384, first + j * 128, last + j * 128, lane);
-      mbar_wait(p_full, g & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
-      tc_fence_after();
-      mma_tmn<8, P_HALF>(tmem_base + O_COL, tmem_base, smem_u32(Vs + st * TILE), 16384, idesc_o, j > j0);
-      umma_commit_e(o_full);
-      umma_commit_e(&v_empty[st]);
-      if (j + 1 < j1) {
-        mbar_wait(o_full, g & 1, wctx, STATUS_TIMEOUT_TMEM_FULL);   // P, where the next scores go, has been read
-        issue_s(j + 1);
+  };
+  auto start = [&]() {
+    Walk k;
+    k.it = 0;
+    fetch(k);
+    return k;
+  };
+  auto next = [&](Walk& k, Item& i) {
+    if (k.w >= n_items) return false;     // can only occur in a CTA's last round
+    const int bh = k.w % BH;
+    i.b = bh / heads;
+    const int h = bh % heads;
+    if (p.head_pairs) {
+      i.h[0] = 2 * h;
+      i.h[1] = 2 * h + 1;
+      i.row[0] = i.row[1] = k.e0.x * 128;
+      i.j0[0] = i.j0[1] = k.e0.y >> 6;
+      i.j1[0] = i.j1[1] = max((k.e0.z + 63) >> 6, i.j0[0] + 1);
+      i.padded = k.e0.w != 0;
+    } else {
+      i.h[0] = i.h[1] = h;
+      i.row[0] = k.e0.x * 256;
+      i.row[1] = i.row[0] + 128;
+      i.j0[0] = k.e0.y;
+      i.j1[0] = k.e0.z;
+      i.j0[1] = k.e0.w;
+      i.j1[1] = k.e1.x;
+      i.padded = k.e1.y != 0;
+    }
+    ++k.it;
+    fetch(k);
+    return true;
+  };
+  // all blocks of an item
+  auto begin_of = [](const Item& i) { return i.j0[1] < i.j1[1] ? min(i.j0[0], i.j0[1]) : i.j0[0]; };
+  auto end_of = [](const Item& i) { return max(i.j1[0], i.j1[1]); };
+
+  if (warp < MFWD_FIRST_SW) {
+    setmaxnreg_dec<MFWD_REGS_IO>();
+    if (warp == 0) {
+      if (lane == 0) {
+        int g = 0;      // key blocks loaded so far (ring position)
+        Walk walk = start();
+        Item item;
+        for (int it = 0; next(walk, item); ++it) {
+          const int kvh = item.h[0] / p.group;
+          mbar_wait(q_empty, (it & 1) ^ 1u, wctx, STATUS_TIMEOUT_PIPE_EMPTY);  // previous item's score MMAs done
+          mbar_arrive_expect_tx(q_full, 2 * Q_TILE);
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int db = 0; db < DB; ++db)     // rows past S: zeros
+              tma_load_4d(Qs + x * Q_TILE + db * 16384, &tq, q_full, db * 64, item.row[x], item.h[x], item.b);
+          const int j1 = end_of(item);
+          for (int j = begin_of(item); j < j1; ++j, ++g) {
+            const int st = g % KS;
+            const uint32_t par = ((g / KS) & 1) ^ 1u;
+            mbar_wait(&k_empty[st], par, wctx, STATUS_TIMEOUT_PIPE_EMPTY);
+            mbar_arrive_expect_tx(&k_full[st], KV_TILE);
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+              tma_load_4d(Ks + st * KV_TILE + db * 8192, &tk, &k_full[st], db * 64, j * 64, kvh, item.b);
+            mbar_wait(&v_empty[st], par, wctx, STATUS_TIMEOUT_PIPE_EMPTY);
+            mbar_arrive_expect_tx(&v_full[st], KV_TILE);
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+              tma_load_4d(Vs + st * KV_TILE + db * 8192, &tv, &v_full[st], db * 64, j * 64, kvh, item.b);
+          }
+        }
+        settle_copies(wctx);
+      }
+    } else if (warp <= 2) {
+      // The MMAs of tile x (whole warp, converged: the MMA / commit helpers elect the issuing lane). Each tile has a warp of its
+      // own, which waits for nothing but its tile: one warp that polled the events of both came 1,100 to 1,700 cycles late. It
+      // walks all blocks of the item; those that only the other tile sees are handed on.
+      // Scores are double buffered: a block's are made while the softmax is at the block before, so neither waits for the other's
+      // latency, nor do the two tiles meet in the same phase.
+      constexpr uint32_t idesc_s = umma_idesc_bf16(128, 64, 0, 0);
+      constexpr uint32_t idesc_o = umma_idesc_bf16(128, D, 0, 1);
+      const int x = warp - 1;
+      const uint32_t s_tmem = tmem_base + x * 128, o_tmem = tmem_base + O_COL + x * D;
+      const uint32_t q_addr = smem_u32(Qs + x * Q_TILE);
+      int g0 = 0;               // ring position of this item's first key block
+      int cx = 0;               // this tile's blocks in earlier items (barrier phases)
+      int had = 0;              // items in which it had blocks (phase of o_empty)
+      Walk walk = start();
+      Item item;
+      for (int it = 0; next(walk, item); ++it) {
+        const int u0 = begin_of(item), u1 = end_of(item);
+        const int j0 = x == 0 ? item.j0[0] : item.j0[1], j1 = x == 0 ? item.j1[0] : item.j1[1];
+        const int *first = p.mask.first + static_cast<size_t>(item.b) * p.S_pad, *last = p.mask.last + static_cast<size_t>(item.b) * p.S_pad;
+        mbar_wait(q_full, it & 1, wctx, STATUS_TIMEOUT_PIPE_FULL);
+        auto scores = [&](int j) {
+          const int g = g0 + j - u0, st = g % KS, n = cx + j - j0, buf = n & 1;
+          mbar_wait(&k_full[st], (g / KS) & 1, wctx, STATUS_TIMEOUT_PIPE_FULL);
+          if (j < j0 || j >= j1) {
+            if (lane == 0) mbar_arrive(&k_empty[st]);
+            return;
+          }
+          if (item.padded) zero_padding(Ks + st * KV_TILE, 64, DB, 8192, first + j * 64, last + j * 64, lane);
+          if (n >= 2) mbar_wait(&o_full[2 * x + buf], ((n - 2) >> 1) & 1, wctx, STATUS_TIMEOUT_TMEM_FULL);   // its P has been read
+          tc_fence_after();
+          mma_kk<D / 16>(s_tmem + buf * 64, q_addr, 16384, smem_u32(Ks + st * KV_TILE), 8192, idesc_s, false);
+          umma_commit_e(&s_full[2 * x + buf]);
+          umma_commit_e(&k_empty[st]);
+        };
+        auto values = [&](int j) {
+          const int g = g0 + j - u0, st = g % KS, n = cx + j - j0, buf = n & 1;
+          mbar_wait(&v_full[st], (g / KS) & 1, wctx, STATUS_TIMEOUT_PIPE_FULL);
+          if (j < j0 || j >= j1) {
+            if (lane == 0) mbar_arrive(&v_empty[st]);
+            return;
+          }
+          if (item.padded) zero_padding(Vs + st * KV_TILE, 64, DB, 8192, first + j * 64, last + j * 64, lane);
+          // the accumulator is overwritten once per item: the previous item's result has been read out of it
+          if (j == j0) mbar_wait(&o_empty[x], (had & 1) ^ 1u, wctx, STATUS_TIMEOUT_SOFTMAX);
+          mbar_wait(&p_full[2 * x + buf], (n >> 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
+          tc_fence_after();
+          mma_tmn<4>(o_tmem, s_tmem + buf * 64, smem_u32(Vs + st * KV_TILE), 8192, idesc_o, j > j0);
+          umma_commit_e(&o_full[2 * x + buf]);
+          umma_commit_e(&v_empty[st]);
+        };
+        scores(u0);
+        if (u0 + 1 < u1) scores(u0 + 1);
+        for (int j = u0; j < u1; ++j) {
+          if (j == max(u1 - 2, u0)) umma_commit_e(q_empty);      // all scores of the item have been issued
+          values(j);
+          if (j + 2 < u1) scores(j + 2);
+        }
+        g0 += u1 - u0;
+        cx += j1 - j0;
+        had += j1 > j0;
       }
     }
   } else {
-    const int half = (warp - 2) >> 2;                       // keys [64 half, + 64) of every block
+    setmaxnreg_inc<MFWD_REGS_SOFTMAX>();
+    const int x = (warp - MFWD_FIRST_SW) >> 2;   // query tile of this warp
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
-    const int row = row_a + r;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_addr = tmem_base + lane_base + half * 64;
-    const uint32_t o_addr = tmem_base + lane_base + O_COL + half * (D / 2);
-    const uint32_t p_addr = tmem_base + lane_base + half * P_HALF;
-    float* const xch_own = xch + half * 128 + r;            // + 256 * parity
-    const float* const xch_other = xch + (half ^ 1) * 128 + r;
-    const int lo = first[row], hi = last[row];
-    const int lo_max = first[row_z], hi_min = last[row_a];  // a block between these is seen whole by every row
-    const float slope2 = DIST ? p.score.slopes[h] * LOG2E_F : 0.f;
-    const float k = CAP || DIST ? 1.f : p.score.sl2;        // what turns the numbers in v[] into exponents
-    const uint64_t k_2 = pack_f32x2(k, k);
-    uint32_t xpar = 0;
-    auto exchange = [&](float v) {
-      xch_own[xpar * 256] = v;
-      named_barrier_sync(1 + quarter, 64);                  // the two warps that share these rows
-      const float o = xch_other[xpar * 256];
-      xpar ^= 1u;
-      return o;
+    const uint32_t s_addr = tmem_base + lane_base + x * 128;
+    const uint32_t o_addr = tmem_base + lane_base + O_COL + x * D;
+    uint8_t* stage = staging + (warp - MFWD_FIRST_SW) * 4096;
+    constexpr bool MAXED = SCORES != BOUNDED;
+    const float sl2 = p.score.sl2, cap2 = p.score.cap2;
+    const float k = SCORES != PLAIN || DIST ? 1.f : sl2;    // what turns the numbers in the registers into exponents
+    const uint64_t k_2 = pack_f32x2(k, k), sl2_2 = pack_f32x2(sl2, sl2);
+    const uint64_t cap_2 = pack_f32x2(cap2, cap2), m2cap_2 = pack_f32x2(-2.f * cap2, -2.f * cap2);
+    // The ends of what a row sees, and what every row of the tile does.
+    struct Rows {
+      int lo, hi, lo_max, hi_min;
+      float slope2;
     };
-    float m = -INFINITY;
-    uint64_t l2 = 0;                                        // two partial sums of this thread's exponentials
-    for (int j = j0; j < j1; ++j) {
-      const int g = j - j0;
-      const int col0 = j * 128 + half * 64;
-      mbar_wait(s_full, g & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
-      tc_fence_after();
-      uint32_t v[2][32];
-      tmem_ld_32x32(s_addr, v[0]);
-      tmem_ld_32x32(s_addr + 32, v[1]);
-      tmem_ld_wait_for(v[0]);
-      tmem_ld_wait_for(v[1]);
-      if (CAP || DIST) {
-        const float dist0 = static_cast<float>(row - col0);
+    auto rows_of = [&](const Item& i) {
+      Rows q;
+      const int *first = p.mask.first + static_cast<size_t>(i.b) * p.S_pad, *last = p.mask.last + static_cast<size_t>(i.b) * p.S_pad;
+      const int a = x == 0 ? i.row[0] : min(i.row[1], p.S_pad - 128);   // (no second tile: loads that nobody uses)
+      q.lo = first[a + r];
+      q.hi = last[a + r];
+      q.lo_max = first[min(a + 127, p.S - 1)];
+      q.hi_min = last[a];
+      q.slope2 = DIST ? -p.score.slopes[i.h[x]] * LOG2E_F : 0.f;
+      return q;
+    };
+    // 32 scores of a row from column col on -> exponents (plain ones: still to be scaled), dead ones -inf
+    auto transform = [&](uint32_t (&v)[32], int col, const Rows& q, int row, bool whole) {
+      if (SCORES != PLAIN || DIST) {
+        const uint64_t slope_2 = pack_f32x2(q.slope2, q.slope2);
+        const float dist0 = static_cast<float>(row - col);
 #pragma unroll
-        for (int e = 0; e < 64; e += 4) {
-          float x[4], y[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) x[u] = __uint_as_float(v[e >> 5][(e & 31) + u]);
-          if (CAP) {
-            float rr[4];
-            sigmoids(x, p.score.sl2, rr);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) y[u] = fmaf(rr[u], -2.f * p.score.cap2, p.score.cap2);
+        for (int e = 0; e < 32; e += 4) {
+          uint64_t y[2] = {pack_u32x2(v[e], v[e + 1]), pack_u32x2(v[e + 2], v[e + 3])};
+          if (SCORES != PLAIN) {
+            uint64_t r0, r1;
+            sigmoids(y[0], y[1], sl2_2, r0, r1);
+            y[0] = fma_f32x2(r0, m2cap_2, cap_2);
+            y[1] = fma_f32x2(r1, m2cap_2, cap_2);
           } else {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) y[u] = x[u] * p.score.sl2;
+            y[0] = mul_f32x2(y[0], sl2_2);
+            y[1] = mul_f32x2(y[1], sl2_2);
           }
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            if (DIST) y[u] = fmaf(fabsf(dist0 - static_cast<float>(e + u)), -slope2, y[u]);
-            v[e >> 5][(e & 31) + u] = __float_as_uint(y[u]);
+          for (int u = 0; u < 2; ++u) {
+            if (DIST)
+              y[u] = fma_f32x2(pack_f32x2(fabsf(dist0 - static_cast<float>(e + 2 * u)), fabsf(dist0 - static_cast<float>(e + 2 * u + 1))),
+                               slope_2, y[u]);
+            const float2 f = unpack_f32x2(y[u]);
+            v[e + 2 * u] = __float_as_uint(f.x);
+            v[e + 2 * u + 1] = __float_as_uint(f.y);
           }
         }
       }
-      if (j * 128 < lo_max || j * 128 + 128 > hi_min) {
-        // some row does not see some key: dead scores become -inf in the registers, then the block takes the same code as every other
-        const int a = lo - col0;
-        const unsigned n = static_cast<unsigned>(hi - lo);
+      if (!whole) {
+        // bits [lo - col, hi - col) of 32
+        const int a = max(q.lo - col, 0), z = q.hi - col;
+        const uint32_t live = (z >= 32 ? 0xffffffffu : (z <= 0 ? 0u : (1u << z) - 1u)) & (a >= 32 ? 0u : 0xffffffffu << a);
 #pragma unroll
-        for (int e = 0; e < 64; ++e)
-          v[e >> 5][e & 31] = static_cast<unsigned>(e - a) < n ? v[e >> 5][e & 31] : 0xff800000u;
+        for (int e = 0; e < 32; ++e) v[e] = (live >> e) & 1u ? v[e] : 0xff800000u;
       }
-      float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 32; e += 2) {
-        mx0 = fmax3(mx0, __uint_as_float(v[0][e]), __uint_as_float(v[0][e + 1]));
-        mx1 = fmax3(mx1, __uint_as_float(v[1][e]), __uint_as_float(v[1][e + 1]));
-      }
-      const float mx = fmaxf(mx0, mx1);
-      const float m_new = fmax3(m, mx, exchange(mx));
-      // the maximum of all keys so far: both threads of a row raise it alike
-      const bool grow = m_new > m;
-      float alpha = 1.f;
-      if (grow) {
-        alpha = (m == -INFINITY) ? 0.f : fast_exp2((m - m_new) * k);
-        l2 = mul_f32x2(l2, pack_f32x2(alpha, alpha));
-        m = m_new;
-      }
-      const float moff = ((m == -INFINITY) ? 0.f : m) * k;
-      const uint64_t moff2 = pack_f32x2(-moff, -moff);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t pk[16];
+    };
+    int cdone = 0;  // blocks of this tile processed in earlier items
+    Walk walk = start();
+    Item item;
+    bool more = next(walk, item);
+    Rows rows = {};
+    if (more) rows = rows_of(item);
+    while (more) {
+      const Item cur = item;
+      const Rows q = rows;
+      more = next(walk, item);
+      if (more) rows = rows_of(item);           // on their way while this item is worked on
+      const int j0 = x == 0 ? cur.j0[0] : cur.j0[1], j1 = x == 0 ? cur.j1[0] : cur.j1[1];
+      const int row = (x == 0 ? cur.row[0] : cur.row[1]) + r;
+      float m = MAXED ? -INFINITY : 0.f;
+      uint64_t l2 = 0, t2 = 0;                  // sums of the probabilities, as they are and as rounded to bf16
+      // 32 exponents -> probabilities, packed, and their sums
+      auto probabilities = [&](const uint32_t (&v)[32], uint32_t (&packed)[16], uint64_t moff2) {
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          const float2 a = unpack_f32x2(fma_f32x2(pack_u32x2(v[c][e], v[c][e + 1]), k_2, moff2));
-          const float p0 = fast_exp2(a.x), p1 = fast_exp2(a.y);
+          const float2 y = MAXED ? unpack_f32x2(fma_f32x2(pack_u32x2(v[e], v[e + 1]), k_2, moff2))
+                                 : make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+          const float p0 = fast_exp2(y.x), p1 = fast_exp2(y.y);
+          const uint32_t w = pack_bf16x2(p0, p1);
           l2 = add_f32x2(l2, pack_f32x2(p0, p1));
-          pk[e >> 1] = pack_bf16x2(p0, p1);
+          t2 = add_f32x2(t2, pack_u32x2(w << 16, w & 0xffff0000u));
+          packed[e >> 1] = w;
         }
-        tmem_st_32x16(p_addr + 16 * c, pk);
-      }
-      if (g > 0 && __any_sync(0xffffffffu, grow)) {
-        // rescale this warp's 32 accumulator rows in tensor memory (warp-collective accesses; rows whose maximum stays get
-        // factor 1), its half of the columns. P V of the previous block is done: this block's scores were issued after it.
-        mbar_wait(o_full, (g - 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
-        tc_fence_after();
-        uint32_t wv[D / 32][16];
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) tmem_ld_32x16(o_addr + 16 * c, wv[c]);
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) tmem_ld_wait_for16(wv[c]);
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) wv[c][e] = __float_as_uint(__uint_as_float(wv[c][e]) * alpha);
-          tmem_st_32x16(o_addr + 16 * c, wv[c]);
-        }
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
-    }
-    const float2 lp = unpack_f32x2(l2);
-    float l = lp.x + lp.y;
-    l += exchange(l);
-    const float inv_l = (l > 0.f) ? 1.f / l : 0.f;
-    mbar_wait(o_full, (j1 - j0 - 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
-    tc_fence_after();
-    uint32_t o[D / 64][32];
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c) tmem_ld_32x32(o_addr + 32 * c, o[c]);
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c) tmem_ld_wait_for(o[c]);
-    if (row < p.S) {
-      const bool seen = lo < hi;
-      __nv_bfloat16* dst = p.O + row * p.o_ss + b * p.o_bs + h * p.o_hs + half * (D / 2);
-      auto two = [&](int c, int e) {
-        return seen ? pack_bf16x2(__uint_as_float(o[c][e]) * inv_l, __uint_as_float(o[c][e + 1]) * inv_l) : 0u;
       };
+      for (int j = j0; j < j1; ++j) {
+        const int c = cdone + j - j0, buf = c & 1;
+        const bool whole = j * 64 >= q.lo_max && j * 64 + 64 <= q.hi_min;   // every row sees every key of the block
+        const uint32_t at = s_addr + buf * 64;
+        mbar_wait(&s_full[2 * x + buf], (c >> 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
+        tc_fence_after();
+        uint32_t v0[32], v1[32], pk[16];
+        tmem_ld_32x32(at, v0);
+        tmem_ld_32x32(at + 32, v1);
+        tmem_ld_wait_for(v0);
+        tmem_ld_wait_for(v1);
+        transform(v0, j * 64, q, row, whole);
+        transform(v1, j * 64 + 32, q, row, whole);
+        uint64_t moff2 = 0;
+        if (MAXED) {
+          float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
+          for (int e = 0; e < 32; e += 2) {
+            mx0 = fmax3(mx0, __uint_as_float(v0[e]), __uint_as_float(v0[e + 1]));
+            mx1 = fmax3(mx1, __uint_as_float(v1[e]), __uint_as_float(v1[e + 1]));
+          }
+          const float m_new = fmaxf(m, fmaxf(mx0, mx1));
+          // The running maximum is raised only when it grew by more than 2^8 (or was still -inf): raising it rescales the
+          // accumulator in tensor memory, which after the first blocks is rare.
+          bool grow = false;
+          float alpha = 1.f;
+          if (m_new > m && (m == -INFINITY || (m_new - m) * k > 8.f)) {
+            grow = true;
+            alpha = (m == -INFINITY) ? 0.f : fast_exp2((m - m_new) * k);
+          }
+          if (j > j0 && __any_sync(0xffffffffu, grow && m != -INFINITY)) {
+            // this warp's 32 accumulator rows (warp-collective accesses; rows whose maximum stays get factor 1, and so do those
+            // that saw nothing yet: they hold zeros). P V of the previous block must be done.
+            mbar_wait(&o_full[2 * x + (buf ^ 1)], ((c - 1) >> 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
+            tc_fence_after();
+            const float a = grow && m != -INFINITY ? alpha : 1.f;
+#pragma unroll 1
+            for (int cc = 0; cc < D; cc += 32) {
+              uint32_t wv[32];
+              tmem_ld_32x32(o_addr + cc, wv);
+              tmem_ld_wait_for(wv);
+              uint32_t lo16[16], hi16[16];
 #pragma unroll
-        for (int e = 0; e < 32; e += 8)
-          *reinterpret_cast<uint4*>(dst + 32 * c + e) = make_uint4(two(c, e), two(c, e + 2), two(c, e + 4), two(c, e + 6));
+              for (int e = 0; e < 16; ++e) {
+                lo16[e] = __float_as_uint(__uint_as_float(wv[e]) * a);
+                hi16[e] = __float_as_uint(__uint_as_float(wv[16 + e]) * a);
+              }
+              tmem_st_32x16(o_addr + cc, lo16);
+              tmem_st_32x16(o_addr + cc + 16, hi16);
+            }
+            tmem_st_wait();
+          }
+          if (grow) {
+            l2 = mul_f32x2(l2, pack_f32x2(alpha, alpha));
+            t2 = mul_f32x2(t2, pack_f32x2(alpha, alpha));
+            m = m_new;
+          }
+          const float moff = ((m == -INFINITY) ? 0.f : m) * k;
+          moff2 = pack_f32x2(-moff, -moff);
+        }
+        // the probabilities go where the scores were: all of those are in registers
+        probabilities(v0, pk, moff2);
+        tmem_st_32x16(at, pk);
+        probabilities(v1, pk, moff2);
+        tmem_st_32x16(at + 16, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * x + buf]);
       }
+      if (j1 > j0) {
+        // The output is normalised by the sum of the probabilities that it was made from, the rounded ones: a row that sees
+        // little but one key has that key's value exactly. The backward recomputes them unrounded and gets the other sum.
+        const float2 lp = unpack_f32x2(l2), tp = unpack_f32x2(t2);
+        const float l = lp.x + lp.y, t = tp.x + tp.y;
+        const float inv = q.lo < q.hi && t > 0.f ? 1.f / t : 0.f;
+        const int c_last = cdone + j1 - j0 - 1;
+        mbar_wait(&o_full[2 * x + (c_last & 1)], (c_last >> 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
+        tc_fence_after();
+        const int row0 = row - lane;
+        __nv_bfloat16* g0 = p.O + row0 * p.o_ss + cur.b * p.o_bs + (x == 0 ? cur.h[0] : cur.h[1]) * p.o_hs;
+        const bool seen = q.lo < q.hi;
+#pragma unroll
+        for (int hf = 0; hf < DB; ++hf) {
+          uint32_t wa[32], wb[32], ow[32];
+          tmem_ld_32x32(o_addr + hf * 64, wa);
+          tmem_ld_32x32(o_addr + hf * 64 + 32, wb);
+          tmem_ld_wait_for(wa);
+          tmem_ld_wait_for(wb);
+          if (hf == DB - 1) {        // the next item's first P V may overwrite the accumulator
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_empty[x]);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            ow[e] = seen ? pack_bf16x2(__uint_as_float(wa[2 * e]) * inv, __uint_as_float(wa[2 * e + 1]) * inv) : 0u;
+            ow[16 + e] = seen ? pack_bf16x2(__uint_as_float(wb[2 * e]) * inv, __uint_as_float(wb[2 * e + 1]) * inv) : 0u;
+          }
+          store_rows_32x64(stage, ow, lane, g0 + hf * 64, p.o_ss, p.S - row0);
+        }
+        if (p.lse != nullptr)
+          p.lse[(static_cast<size_t>(cur.b) * p.nh + (x == 0 ? cur.h[0] : cur.h[1])) * p.S_pad + row] =
+              l > 0.f ? m * k + log2f(l) : (l == 0.f ? INFINITY : l);
+      }
+      cdone += j1 - j0;
     }
-    if (half == 0 && p.lse != nullptr)
-      p.lse[static_cast<size_t>(bh) * p.S_pad + row] = l > 0.f ? m * k + log2f(l) : (l == 0.f ? INFINITY : l);
   }
 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem_base, 256);
+  if (warp == 1) tmem_dealloc(tmem_base, 512);
 }
 
-template <int D, bool CAP, bool DIST>
+template <int D, int SCORES, bool DIST>
 int launch_fwd(const CUtensorMap* tq, const CUtensorMap* tk, const CUtensorMap* tv, const MaskedFwdParams& p,
                cudaStream_t stream) {
   static gfs_host::SmemLimit limit;
   constexpr int smem = MFwdShape<D>::SMEM;
-  if (!limit.raise(masked_fwd_kernel<D, CAP, DIST>, smem)) return -10;
-  const int n_tiles = p.S_pad / 128;
-  gfs_host::launch_pdl(masked_fwd_kernel<D, CAP, DIST>, dim3(static_cast<unsigned>(n_tiles) * p.B * p.nh),
-                       dim3(MFWD_THREADS), smem, stream, *tq, *tk, *tv, p, n_tiles);
+  if (!limit.raise(masked_fwd_kernel<D, SCORES, DIST>, smem)) return -10;
+  const int tiles = p.S_pad / 128;
+  const int n_levels = p.head_pairs ? tiles : (tiles + 1) / 2;
+  const int n_items = n_levels * p.B * (p.head_pairs ? p.nh / 2 : p.nh);
+  gfs_host::launch_pdl(masked_fwd_kernel<D, SCORES, DIST>, dim3(std::min(n_items, gfs_host::sm_count())), dim3(MFWD_THREADS),
+                       smem, stream, *tq, *tk, *tv, p, n_levels, n_items);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
-template <int D>
+template <int D, bool DIST>
 int launch_fwd_scores(const CUtensorMap* tq, const CUtensorMap* tk, const CUtensorMap* tv, const MaskedFwdParams& p,
-                      bool cap, cudaStream_t stream) {
-  const bool dist = p.score.slopes != nullptr;
-  if (cap) return dist ? launch_fwd<D, true, true>(tq, tk, tv, p, stream) : launch_fwd<D, true, false>(tq, tk, tv, p, stream);
-  return dist ? launch_fwd<D, false, true>(tq, tk, tv, p, stream) : launch_fwd<D, false, false>(tq, tk, tv, p, stream);
+                      cudaStream_t stream) {
+  if (p.score.cap2 <= 0.f) return launch_fwd<D, PLAIN, DIST>(tq, tk, tv, p, stream);
+  return p.score.cap2 <= BOUNDED_CAP2 ? launch_fwd<D, BOUNDED, DIST>(tq, tk, tv, p, stream)
+                                      : launch_fwd<D, CAPPED, DIST>(tq, tk, tv, p, stream);
 }
 
 }  // namespace
@@ -475,16 +680,18 @@ int gfs_attention_mask(const void* ids, int ids64, const void* prefix, int B, in
   const MaskLayout l = mask_layout(B, S);
   const MaskArgs a{ids, static_cast<const uint8_t*>(prefix), ids64, S, (S + 127) / 128 * 128, window > S ? 0 : window, causal,
                    o + l.first, o + l.last, o + l.qfirst, o + l.qlast, o + l.padded, o + l.positions,
-                   reinterpret_cast<int4*>(o + l.plan_q), reinterpret_cast<int4*>(o + l.plan_k)};
+                   reinterpret_cast<int4*>(o + l.plan_q), reinterpret_cast<int4*>(o + l.plan_k),
+                   reinterpret_cast<int4*>(o + l.pairs)};
   gfs_host::launch_pdl(attention_mask_kernel, dim3(B), dim3(MASK_THREADS), 0, static_cast<cudaStream_t>(stream), a);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 
-// offsets[9]: where the buffer of a mask has first, last, qfirst, qlast, plan_q, plan_k, padded and positions, and its length.
+// offsets[10]: where the buffer of a mask has first, last, qfirst, qlast, plan_q, plan_k, pairs, padded and positions, and its
+// length.
 void gfs_attention_mask_layout(int B, int S, long long* offsets) {
   const MaskLayout l = mask_layout(B, S);
-  const size_t at[9] = {l.first, l.last, l.qfirst, l.qlast, l.plan_q, l.plan_k, l.padded, l.positions, l.end};
-  for (int i = 0; i < 9; ++i) offsets[i] = static_cast<long long>(at[i]);
+  const size_t at[10] = {l.first, l.last, l.qfirst, l.qlast, l.plan_q, l.plan_k, l.pairs, l.padded, l.positions, l.end};
+  for (int i = 0; i < 10; ++i) offsets[i] = static_cast<long long>(at[i]);
 }
 
 // q [B, nh, S, D], k and v [B, nkv, S, D], out like q; strides: 12 element strides {q, k, v, out} x {seq, batch, head}.
@@ -501,22 +708,24 @@ int gfs_masked_attention_fwd(const void* q, const void* k, const void* v, void* 
   const int S_pad = (S + 127) / 128 * 128;
   if (static_cast<long long>(S_pad / 128) * B * nh > 0x7fffffffll) return -1;
   const CUtensorMap* tq = make_map(q, D, S, nh, B, strides + 0, 128);
-  const CUtensorMap* tk = make_map(k, D, S, nkv, B, strides + 3, 128);
-  const CUtensorMap* tv = make_map(v, D, S, nkv, B, strides + 6, 128);
+  const CUtensorMap* tk = make_map(k, D, S, nkv, B, strides + 3, 64);
+  const CUtensorMap* tv = make_map(v, D, S, nkv, B, strides + 6, 64);
   if (!tq || !tk || !tv) return -3;
   MaskedFwdParams p;
   p.O = static_cast<__nv_bfloat16*>(out);
   p.o_ss = strides[9]; p.o_bs = strides[10]; p.o_hs = strides[11];
   p.lse = static_cast<float*>(lse);
   p.S = S; p.S_pad = S_pad; p.B = B; p.nh = nh; p.group = nh / nkv;
+  p.head_pairs = p.group % 2 == 0;
   p.score.sl2 = cap > 0.f ? 2.f * scale * LOG2E_F / cap : scale * LOG2E_F;
   p.score.cap2 = cap * LOG2E_F;
   p.score.slopes = static_cast<const float*>(slopes);
   p.mask = mask_view(mask, B, S);
   p.status = gfs_host::status_words();
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  return D == 64 ? launch_fwd_scores<64>(tq, tk, tv, p, cap > 0.f, stream)
-                 : launch_fwd_scores<128>(tq, tk, tv, p, cap > 0.f, stream);
+  if (slopes != nullptr)
+    return D == 64 ? launch_fwd_scores<64, true>(tq, tk, tv, p, stream) : launch_fwd_scores<128, true>(tq, tk, tv, p, stream);
+  return D == 64 ? launch_fwd_scores<64, false>(tq, tk, tv, p, stream) : launch_fwd_scores<128, false>(tq, tk, tv, p, stream);
 }
 
 }  // extern "C"

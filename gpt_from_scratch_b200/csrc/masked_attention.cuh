@@ -17,20 +17,16 @@ struct MaskView {
   const int *first, *last;     // [B, S_pad]: the keys that a query sees
   const int *qfirst, *qlast;   // [B, S_pad]: the queries that see a key
   const int4 *plan_q, *plan_k; // [B, S_pad / 128]: the tiles of 128 queries (keys), those that see (are seen by) most first
+  const int4* pairs;           // [B, ceil(S_pad / 256), 2]: the same for pairs of query tiles
   const int* padded;           // [B]: the sequence has padding
 };
-// An entry of a plan: the tile, the first row that any of its rows sees (for keys: is seen by), one past the last.
-struct TilePlan {
-  int tile, lo, hi;
-};
-__device__ __forceinline__ TilePlan load_plan(const int4* p) {
-  const int4 e = *p;
-  return TilePlan{e.x, e.y, e.z};
-}
+// An entry of a plan: {tile, the first row that any of its rows sees (for keys: is seen by), one past the last, padded}.
+// Of the pairs: {pair, blocks [a0, a1) of 64 keys of its first tile, b0}, {b1 of its second tile, padded, 0, 0}; the blocks of both
+// are one stretch without a gap, at least one each; b0 == b1: there is no second tile.
 
 // The parts of the buffer that gfs_attention_mask fills: int32 offsets.
 struct MaskLayout {
-  size_t first, last, qfirst, qlast, plan_q, plan_k, padded, positions, end;
+  size_t first, last, qfirst, qlast, plan_q, plan_k, pairs, padded, positions, end;
 };
 __host__ __device__ inline MaskLayout mask_layout(int B, int S) {
   const size_t S_pad = (static_cast<size_t>(S) + 127) / 128 * 128;
@@ -42,7 +38,8 @@ __host__ __device__ inline MaskLayout mask_layout(int B, int S) {
   l.qlast = 3 * n;
   l.plan_q = 4 * n;
   l.plan_k = l.plan_q + plan;
-  l.positions = l.plan_k + plan;
+  l.pairs = l.plan_k + plan;
+  l.positions = l.pairs + B * ((S_pad / 128 + 1) / 2) * 8;
   l.padded = l.positions + static_cast<size_t>(B) * S;
   l.end = l.padded + B;
   return l;
@@ -51,7 +48,7 @@ inline MaskView mask_view(const void* buffer, int B, int S) {
   const int* m = static_cast<const int*>(buffer);
   const MaskLayout l = mask_layout(B, S);
   return MaskView{m + l.first, m + l.last, m + l.qfirst, m + l.qlast, reinterpret_cast<const int4*>(m + l.plan_q),
-                  reinterpret_cast<const int4*>(m + l.plan_k), m + l.padded};
+                  reinterpret_cast<const int4*>(m + l.plan_k), reinterpret_cast<const int4*>(m + l.pairs), m + l.padded};
 }
 
 // The softmax's exponents are base 2: score = log2(e) (scale q k, or cap tanh(scale q k / cap)) - slope log2(e) |i - j|.
@@ -67,20 +64,21 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return d;
 }
 
-// r = 1 / (1 + 2^(sl2 x)) of four scores: tanh = 1 - 2 r, its derivative 4 r (1 - r). The absolute error counts here
-// (the score is an exponent), and it is that of r, a few 2^-24: the approximate tanh instruction is off by up to 2^-11 of the
-// value, 0.02 for a score of 40. Four exponentials and one reciprocal, of the product of the four denominators: it stays in range as
-// exponents are cut off at 30, where tanh is 1 to 32 bits.
-__device__ __forceinline__ void sigmoids(const float (&x)[4], float sl2, float (&r)[4]) {
-  float d[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) d[i] = 1.f + fast_exp2(min_nan(x[i] * sl2, 30.f));
-  const float a = d[0] * d[1], b = d[2] * d[3], inv = fast_rcp(a * b);
-  const float ra = inv * b, rb = inv * a;
-  r[0] = ra * d[1];
-  r[1] = ra * d[0];
-  r[2] = rb * d[3];
-  r[3] = rb * d[2];
+// r = 1 / (1 + 2^(sl2 x)) of four scores, as two pairs: tanh = 1 - 2 r, its derivative 4 r (1 - r). The absolute error counts
+// here (the score is an exponent), and it is that of r, a few 2^-24: the approximate tanh instruction is off by up to
+// 2^-11 of the value, 0.02 for a score of 40. Four exponentials and one reciprocal, of the product of the four denominators: it
+// stays in range as exponents are cut off at 30, where tanh is 1 to 32 bits. In pairs (one instruction of the FMA pipe for
+// two scores) 5 instructions a score.
+__device__ __forceinline__ void sigmoids(uint64_t x0, uint64_t x1, uint64_t sl2, uint64_t& r0, uint64_t& r1) {
+  const float2 u0 = unpack_f32x2(mul_f32x2(x0, sl2)), u1 = unpack_f32x2(mul_f32x2(x1, sl2));
+  const uint64_t one = pack_f32x2(1.f, 1.f);
+  const uint64_t d0 = add_f32x2(pack_f32x2(fast_exp2(min_nan(u0.x, 30.f)), fast_exp2(min_nan(u0.y, 30.f))), one);
+  const uint64_t d1 = add_f32x2(pack_f32x2(fast_exp2(min_nan(u1.x, 30.f)), fast_exp2(min_nan(u1.y, 30.f))), one);
+  const float2 pr = unpack_f32x2(mul_f32x2(d0, d1));
+  const float inv = fast_rcp(pr.x * pr.y);
+  const uint64_t q = pack_f32x2(inv * pr.y, inv * pr.x);      // 1 / (d0 d1), elementwise
+  r0 = mul_f32x2(q, d1);
+  r1 = mul_f32x2(q, d0);
 }
 
 // Zeros in the rows of a tile (swizzled blocks of 64 columns, `rows` rows of 128 bytes, `blocks` of them block_bytes apart) whose

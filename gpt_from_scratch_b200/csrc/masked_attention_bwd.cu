@@ -407,7 +407,7 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
           const unsigned width = static_cast<unsigned>(hi - lo);
           // Chunks seen in part turn their dead scores into -inf in the registers, which makes both P and dS exact
           // zeros (dvec and dP are finite: padding was zeroed), and run the same code as the others.
-          if (!CAP && !DIST && kind == 1) {
+          if (!CAP && kind == 1) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) xv[e] = static_cast<unsigned>(e - a) < width ? xv[e] : 0xff800000u;
           }
@@ -415,55 +415,39 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
           const float* st_dv = st_lse + 64;
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            float ls[4], dv[4];
+            uint64_t ls[2], dv[2];
             if (MODE == 0) {   // per-column statistics of the streamed query tile (same address in all lanes)
-              *reinterpret_cast<float4*>(ls) = *reinterpret_cast<const float4*>(st_lse + e);
-              *reinterpret_cast<float4*>(dv) = *reinterpret_cast<const float4*>(st_dv + e);
+              const float4 l4 = *reinterpret_cast<const float4*>(st_lse + e);
+              const float4 d4 = *reinterpret_cast<const float4*>(st_dv + e);
+              ls[0] = pack_f32x2(l4.x, l4.y); ls[1] = pack_f32x2(l4.z, l4.w);
+              dv[0] = pack_f32x2(d4.x, d4.y); dv[1] = pack_f32x2(d4.z, d4.w);
             } else {
-              ls[0] = ls[1] = ls[2] = ls[3] = row_lse;
-              dv[0] = dv[1] = dv[2] = dv[3] = row_dvec;
+              ls[0] = ls[1] = pack_f32x2(row_lse, row_lse);
+              dv[0] = dv[1] = pack_f32x2(row_dvec, row_dvec);
             }
-            float pr[4], slope[4];     // probabilities; derivative of the capped score / 4
-            if (CAP || DIST) {
-              float x[4], y[4];
+            uint64_t r[2];             // of capped scores: their derivative is 4 r (1 - r)
+            if (CAP) sigmoids(pack_u32x2(xv[e], xv[e + 1]), pack_u32x2(xv[e + 2], xv[e + 3]), pack_f32x2(sl2, sl2), r[0], r[1]);
 #pragma unroll
-              for (int u = 0; u < 4; ++u) x[u] = __uint_as_float(xv[e + u]);
-              if (CAP) {
-                float rr[4];
-                sigmoids(x, sl2, rr);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                  y[u] = fmaf(rr[u], -2.f * cap2, cap2);
-                  slope[u] = fmaf(-rr[u], rr[u], rr[u]);
-                }
-              } else {
-#pragma unroll
-                for (int u = 0; u < 4; ++u) y[u] = x[u] * sl2;
+            for (int u = 0; u < 2; ++u) {
+              // lse - score, formed negated (the exponential turns the sign back), two columns per instruction
+              uint64_t z = CAP ? fma_f32x2(r[u], pack_f32x2(2.f * cap2, 2.f * cap2), add_f32x2(ls[u], pack_f32x2(-cap2, -cap2)))
+                               : fma_f32x2(pack_u32x2(xv[e + 2 * u], xv[e + 2 * u + 1]), neg_sl2, ls[u]);
+              if (DIST) {
+                const float at = dist0 - static_cast<float>(e + 2 * u);
+                z = fma_f32x2(pack_f32x2(fabsf(at), fabsf(at - 1.f)), pack_f32x2(slope2, slope2), z);
               }
-#pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                if (DIST) y[u] = fmaf(fabsf(dist0 - static_cast<float>(e + u)), -slope2, y[u]);
-                if (kind == 1 && static_cast<unsigned>(e + u - a) >= width) y[u] = -INFINITY;
-                pr[u] = fast_exp2(y[u] - ls[u]);
+              float2 zz = unpack_f32x2(z);
+              if (CAP && kind == 1) {    // (other scores are made -inf before)
+                zz.x = static_cast<unsigned>(e + 2 * u - a) < width ? zz.x : INFINITY;
+                zz.y = static_cast<unsigned>(e + 2 * u + 1 - a) < width ? zz.y : INFINITY;
               }
-            } else {
-#pragma unroll
-              for (int u = 0; u < 4; u += 2) {
-                // 2^(x scale log2(e) - lse), two columns per instruction: formed negated, the exponential turns the sign back
-                const float2 z = unpack_f32x2(fma_f32x2(pack_u32x2(xv[e + u], xv[e + u + 1]), neg_sl2,
-                                                        pack_f32x2(ls[u], ls[u + 1])));
-                pr[u] = fast_exp2(-z.x);
-                pr[u + 1] = fast_exp2(-z.y);
-              }
-            }
-#pragma unroll
-            for (int u = 0; u < 4; u += 2) {
-              const uint64_t dy = fma_f32x2(pack_f32x2(dv[u], dv[u + 1]), neg_one, pack_u32x2(yv[e + u], yv[e + u + 1]));
-              uint64_t d2 = mul_f32x2(pack_f32x2(pr[u], pr[u + 1]), dy);
-              if (CAP) d2 = mul_f32x2(d2, pack_f32x2(4.f * slope[u], 4.f * slope[u + 1]));
+              const float p0 = fast_exp2(-zz.x), p1 = fast_exp2(-zz.y);
+              const uint64_t dy = fma_f32x2(dv[u], neg_one, pack_u32x2(yv[e + 2 * u], yv[e + 2 * u + 1]));
+              uint64_t d2 = mul_f32x2(pack_f32x2(p0, p1), dy);
+              if (CAP) d2 = mul_f32x2(d2, fma_f32x2(mul_f32x2(r[u], neg_one), r[u], r[u]));   // its 4: in the result's scale
               const float2 d = unpack_f32x2(d2);
-              if (MODE == 0) pp[(e + u) >> 1] = pack_bf16x2(pr[u], pr[u + 1]);
-              dd[(e + u) >> 1] = pack_bf16x2(d.x, d.y);
+              if (MODE == 0) pp[(e >> 1) + u] = pack_bf16x2(p0, p1);
+              dd[(e >> 1) + u] = pack_bf16x2(d.x, d.y);
             }
           }
         }
@@ -494,7 +478,7 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
       constexpr int NC = (MODE == 0) ? D / 64 : 1;    // 32-column chunks per warp
       const int c0 = (MODE == 0) ? half * (D / 2) : (D == 128 ? group * 64 + half * 32 : half * 32);
       const bool is_dv = MODE == 0 && group == 1;
-      const float out_scale = is_dv ? 1.f : p.scale;
+      const float out_scale = is_dv ? 1.f : (CAP ? 4.f : 1.f) * p.scale;
       const bool seen = lo < hi;                       // padding: zeros, whatever its own rows held
       const long long o_ss = is_dv ? p.o2_ss : p.o1_ss;
       __nv_bfloat16* out = is_dv ? p.out2 + row0 * p.o2_ss + b * p.o2_bs + h * p.o2_hs
@@ -575,7 +559,7 @@ masked_dkv_kernel(const float* partial, int parts, __nv_bfloat16* __restrict__ d
 // Into how many parts the heads of a group are dealt for dK and dV.
 int group_parts(int tiles, int B, int nkv, int group) {
   int parts = 1;
-  while (parts < 4 && group % (2 * parts) == 0 && static_cast<long long>(tiles) * B * nkv * parts < 4ll * gfs_host::sm_count())
+  while (parts < 4 && group % (2 * parts) == 0 && static_cast<long long>(tiles) * B * nkv * parts < 2ll * gfs_host::sm_count())
     parts *= 2;
   return tiles > 1 ? parts : 1;
 }

@@ -57,9 +57,9 @@ class AttentionMask:
 @functools.lru_cache(maxsize=256)
 def _layout(B: int, S: int) -> dict[str, int]:
     """Where a mask's buffer has its parts, and its length."""
-    at = (ctypes.c_longlong * 9)()
+    at = (ctypes.c_longlong * 10)()
     _lib.lib().gfs_attention_mask_layout(B, S, at)
-    return dict(zip(("first", "last", "qfirst", "qlast", "plan_q", "plan_k", "padded", "positions", "end"), at))
+    return dict(zip(("first", "last", "qfirst", "qlast", "plan_q", "plan_k", "pairs", "padded", "positions", "end"), at))
 
 
 def _pad128(S: int) -> int:
@@ -85,7 +85,7 @@ def _mask_reference(batch, seq_len, causal, ids, prefix, window, device):
     if window is not None:
         first = torch.maximum(first, at - window + 1)
     if ids is not None:
-        first, last = torch.where(ids < 0, start, first), torch.where(ids < 0, start, last)
+        first, last = torch.where(ids < 0, at, first), torch.where(ids < 0, at, last)
     return AttentionMask(batch, S, device, parts=(first.int(), last.int(), (at - start).int()))
 
 
