@@ -190,17 +190,28 @@ struct MaskedFwdParams {
   uint32_t* status;
 };
 
-constexpr int MFWD_FIRST_SW = 4;                    // warps 0: TMA, 1 and 2: the MMAs of a tile, 3: idle; then the softmax warps
-constexpr int MFWD_THREADS = 32 * (MFWD_FIRST_SW + 8);
-// 384 threads x 168 at the launch = 128 x 72 + 256 x 216: a softmax thread holds the 128 scores of its row.
+constexpr int MFWD_FIRST_SW = 4;                    // warps 0: TMA, 1 and 2: the MMAs of a tile, 3: items and their queries; then the softmax warps
+constexpr int MFWD_SW = 8;                          // four per tile, a row per thread
+constexpr int MFWD_THREADS = 32 * (MFWD_FIRST_SW + MFWD_SW);
+// 384 threads x 168 at the launch = 128 x 72 + 256 x 216: a softmax thread holds the scores of two blocks of its row.
 constexpr int MFWD_REGS_IO = 72, MFWD_REGS_SOFTMAX = 216;
+// A work item, as warp 3 puts it into shared memory one ahead of the others: nobody else divides or waits for the plans.
+struct alignas(16) FwdItem {
+  int more;                    // 0: there are no further items
+  int b, padded;
+  int h[2], row[2];            // heads and first query rows of the two tiles
+  int j0[2], j1[2];            // their blocks of 64 keys; j0 == j1: there is no second tile
+  int lo_max[2], hi_min[2];    // what every row of a tile sees
+  float slope2[2];             // - slope log2(e)
+  int lo[2][128], hi[2][128];  // what the rows see
+};
 template <int D>
 struct MFwdShape {
   static constexpr int DB = D / 64;
   static constexpr int Q_TILE = DB * 16384, KV_TILE = DB * 8192;    // 128 queries, 64 keys
   static constexpr int KS = D == 64 ? 8 : 4;        // stages of K and V
-  static constexpr int STAGING = 8 * 4096;          // to transpose the output rows through
-  static constexpr int SMEM = 2 * Q_TILE + 2 * KS * KV_TILE + STAGING + 512;
+  static constexpr int STAGING = MFWD_SW * 2048;    // to transpose the output rows through
+  static constexpr int SMEM = 2 * Q_TILE + 2 * KS * KV_TILE + STAGING + 2 * sizeof(FwdItem) + 512;
 };
 // Scores: as they are, capped with a bound that the running maximum may be left out for, capped.
 enum Scores { PLAIN = 0, BOUNDED = 1, CAPPED = 2 };
@@ -220,10 +231,11 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
   uint8_t* Ks = Qs + 2 * Q_TILE;             // [KS]
   uint8_t* Vs = Ks + KS * KV_TILE;           // [KS]
   uint8_t* staging = Vs + KS * KV_TILE;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + Shape::STAGING);
-  uint64_t* q_full = bars;
-  uint64_t* q_empty = bars + 1;
-  uint64_t* k_full = bars + 2;               // [KS]
+  FwdItem* items = reinterpret_cast<FwdItem*>(staging + Shape::STAGING);   // [2]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(items + 2);
+  uint64_t* q_full = bars;                   // [tile]
+  uint64_t* q_empty = bars + 2;
+  uint64_t* k_full = bars + 4;               // [KS]
   uint64_t* k_empty = k_full + KS;
   uint64_t* v_full = k_empty + KS;
   uint64_t* v_empty = v_full + KS;
@@ -231,7 +243,9 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
   uint64_t* p_full = s_full + 4;
   uint64_t* o_full = p_full + 4;             // P V of the buffer is done
   uint64_t* o_empty = o_full + 4;            // [tile]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
+  uint64_t* i_full = o_empty + 2;            // [2]
+  uint64_t* i_empty = i_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(i_empty + 2);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -241,8 +255,7 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
     return;
   }
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 2);
+    for (int i = 0; i < 4; ++i) mbar_init(&bars[i], 1);
     for (int i = 0; i < KS; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 2);
@@ -251,10 +264,14 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[i], MFWD_SW / 2);
       mbar_init(&o_full[i], 1);
     }
-    for (int x = 0; x < 2; ++x) mbar_init(&o_empty[x], 4);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&o_empty[x], MFWD_SW / 2);
+      mbar_init(&i_full[x], 32);
+      mbar_init(&i_empty[x], 3 + MFWD_SW);
+    }
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tq);
@@ -273,102 +290,51 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
   const uint32_t tmem_base = *tmem_slot;
   WaitCtx wctx{abort_flag, p.status, GFS_WAIT_LIMIT_NS};
 
-  // Items: the widest first, dealt to the CTAs in a snake; all barrier parities run on counters that continue across
-  // items. The plan of the next item is on its way while one is worked on.
-  const int heads = p.head_pairs ? p.nh / 2 : p.nh;
-  const int BH = p.B * heads;
-  const int G = static_cast<int>(gridDim.x);
-  struct Item {
-    int b, h[2], row[2];        // batch, heads and first query rows of the two tiles
-    int j0[2], j1[2];           // their blocks of 64 keys; j0 == j1: there is no second tile
-    bool padded;
+  // Items: the widest first, dealt to the CTAs in a snake; all barrier parities run on counters that continue across items.
+  // What a warp wants of the it-th item it copies out of its slot, then it releases the slot.
+  auto item_of = [&](int it) -> const FwdItem& {
+    mbar_wait(&i_full[it & 1], (it >> 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
+    return items[it & 1];
   };
-  struct Walk {
-    int it, w;
-    int4 e0, e1;
+  auto release_item = [&](int it) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&i_empty[it & 1]);
   };
-  auto fetch = [&](Walk& k) {
-    k.w = k.it * G + ((k.it & 1) ? G - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
-    if (k.w < n_items) {
-      const size_t at = static_cast<size_t>((k.w % BH) / heads) * n_levels + k.w / BH;
-      if (p.head_pairs) {
-        k.e0 = p.mask.plan_q[at];
-      } else {
-        k.e0 = p.mask.pairs[2 * at];
-        k.e1 = p.mask.pairs[2 * at + 1];
-      }
-    }
+  struct Blocks {
+    int u0, u1;      // all blocks of the item
   };
-  auto start = [&]() {
-    Walk k;
-    k.it = 0;
-    fetch(k);
-    return k;
+  auto blocks_of = [](const FwdItem& i) {
+    return Blocks{i.j0[1] < i.j1[1] ? min(i.j0[0], i.j0[1]) : i.j0[0], max(i.j1[0], i.j1[1])};
   };
-  auto next = [&](Walk& k, Item& i) {
-    if (k.w >= n_items) return false;     // can only occur in a CTA's last round
-    const int bh = k.w % BH;
-    i.b = bh / heads;
-    const int h = bh % heads;
-    if (p.head_pairs) {
-      i.h[0] = 2 * h;
-      i.h[1] = 2 * h + 1;
-      i.row[0] = i.row[1] = k.e0.x * 128;
-      i.j0[0] = i.j0[1] = k.e0.y >> 6;
-      i.j1[0] = i.j1[1] = max((k.e0.z + 63) >> 6, i.j0[0] + 1);
-      i.padded = k.e0.w != 0;
-    } else {
-      i.h[0] = i.h[1] = h;
-      i.row[0] = k.e0.x * 256;
-      i.row[1] = i.row[0] + 128;
-      i.j0[0] = k.e0.y;
-      i.j1[0] = k.e0.z;
-      i.j0[1] = k.e0.w;
-      i.j1[1] = k.e1.x;
-      i.padded = k.e1.y != 0;
-    }
-    ++k.it;
-    fetch(k);
-    return true;
-  };
-  // all blocks of an item
-  auto begin_of = [](const Item& i) { return i.j0[1] < i.j1[1] ? min(i.j0[0], i.j0[1]) : i.j0[0]; };
-  auto end_of = [](const Item& i) { return max(i.j1[0], i.j1[1]); };
 
   if (warp < MFWD_FIRST_SW) {
     setmaxnreg_dec<MFWD_REGS_IO>();
     if (warp == 0) {
-      if (lane == 0) {
-        int g = 0;      // key blocks loaded so far (ring position)
-        Walk walk = start();
-        Item item;
-        for (int it = 0; next(walk, item); ++it) {
-          const int kvh = item.h[0] / p.group;
-          mbar_wait(q_empty, (it & 1) ^ 1u, wctx, STATUS_TIMEOUT_PIPE_EMPTY);  // previous item's score MMAs done
-          mbar_arrive_expect_tx(q_full, 2 * Q_TILE);
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int db = 0; db < DB; ++db)     // rows past S: zeros
-              tma_load_4d(Qs + x * Q_TILE + db * 16384, &tq, q_full, db * 64, item.row[x], item.h[x], item.b);
-          const int j1 = end_of(item);
-          for (int j = begin_of(item); j < j1; ++j, ++g) {
+      int g = 0;      // key blocks loaded so far (ring position)
+      for (int it = 0;; ++it) {
+        const FwdItem& item = item_of(it);
+        if (item.more == 0 || *abort_flag) break;
+        const int bb = item.b, kvh = item.h[0] / p.group;
+        const Blocks u = blocks_of(item);
+        release_item(it);
+        if (lane == 0) {
+          for (int j = u.u0; j < u.u1; ++j, ++g) {
             const int st = g % KS;
             const uint32_t par = ((g / KS) & 1) ^ 1u;
             mbar_wait(&k_empty[st], par, wctx, STATUS_TIMEOUT_PIPE_EMPTY);
             mbar_arrive_expect_tx(&k_full[st], KV_TILE);
 #pragma unroll
             for (int db = 0; db < DB; ++db)
-              tma_load_4d(Ks + st * KV_TILE + db * 8192, &tk, &k_full[st], db * 64, j * 64, kvh, item.b);
+              tma_load_4d(Ks + st * KV_TILE + db * 8192, &tk, &k_full[st], db * 64, j * 64, kvh, bb);
             mbar_wait(&v_empty[st], par, wctx, STATUS_TIMEOUT_PIPE_EMPTY);
             mbar_arrive_expect_tx(&v_full[st], KV_TILE);
 #pragma unroll
             for (int db = 0; db < DB; ++db)
-              tma_load_4d(Vs + st * KV_TILE + db * 8192, &tv, &v_full[st], db * 64, j * 64, kvh, item.b);
+              tma_load_4d(Vs + st * KV_TILE + db * 8192, &tv, &v_full[st], db * 64, j * 64, kvh, bb);
           }
         }
-        settle_copies(wctx);
       }
+      if (lane == 0) settle_copies(wctx);
     } else if (warp <= 2) {
       // The MMAs of tile x (whole warp, converged: the MMA / commit helpers elect the issuing lane). Each tile has a warp of its
       // own, which waits for nothing but its tile: one warp that polled the events of both came 1,100 to 1,700 cycles late. It
@@ -383,13 +349,15 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       int g0 = 0;               // ring position of this item's first key block
       int cx = 0;               // this tile's blocks in earlier items (barrier phases)
       int had = 0;              // items in which it had blocks (phase of o_empty)
-      Walk walk = start();
-      Item item;
-      for (int it = 0; next(walk, item); ++it) {
-        const int u0 = begin_of(item), u1 = end_of(item);
-        const int j0 = x == 0 ? item.j0[0] : item.j0[1], j1 = x == 0 ? item.j1[0] : item.j1[1];
+      for (int it = 0;; ++it) {
+        const FwdItem& item = item_of(it);
+        if (item.more == 0 || *abort_flag) break;
+        const int u0 = blocks_of(item).u0, u1 = blocks_of(item).u1;
+        const int j0 = item.j0[x], j1 = item.j1[x];
+        const bool padded = item.padded != 0;
         const int *first = p.mask.first + static_cast<size_t>(item.b) * p.S_pad, *last = p.mask.last + static_cast<size_t>(item.b) * p.S_pad;
-        mbar_wait(q_full, it & 1, wctx, STATUS_TIMEOUT_PIPE_FULL);
+        release_item(it);
+        mbar_wait(&q_full[x], it & 1, wctx, STATUS_TIMEOUT_PIPE_FULL);
         auto scores = [&](int j) {
           const int g = g0 + j - u0, st = g % KS, n = cx + j - j0, buf = n & 1;
           mbar_wait(&k_full[st], (g / KS) & 1, wctx, STATUS_TIMEOUT_PIPE_FULL);
@@ -397,7 +365,7 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
             if (lane == 0) mbar_arrive(&k_empty[st]);
             return;
           }
-          if (item.padded) zero_padding(Ks + st * KV_TILE, 64, DB, 8192, first + j * 64, last + j * 64, lane);
+          if (padded) zero_padding(Ks + st * KV_TILE, 64, DB, 8192, first + j * 64, last + j * 64, lane);
           if (n >= 2) mbar_wait(&o_full[2 * x + buf], ((n - 2) >> 1) & 1, wctx, STATUS_TIMEOUT_TMEM_FULL);   // its P has been read
           tc_fence_after();
           mma_kk<D / 16>(s_tmem + buf * 64, q_addr, 16384, smem_u32(Ks + st * KV_TILE), 8192, idesc_s, false);
@@ -411,7 +379,7 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
             if (lane == 0) mbar_arrive(&v_empty[st]);
             return;
           }
-          if (item.padded) zero_padding(Vs + st * KV_TILE, 64, DB, 8192, first + j * 64, last + j * 64, lane);
+          if (padded) zero_padding(Vs + st * KV_TILE, 64, DB, 8192, first + j * 64, last + j * 64, lane);
           // the accumulator is overwritten once per item: the previous item's result has been read out of it
           if (j == j0) mbar_wait(&o_empty[x], (had & 1) ^ 1u, wctx, STATUS_TIMEOUT_SOFTMAX);
           mbar_wait(&p_full[2 * x + buf], (n >> 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
@@ -423,7 +391,7 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
         scores(u0);
         if (u0 + 1 < u1) scores(u0 + 1);
         for (int j = u0; j < u1; ++j) {
-          if (j == max(u1 - 2, u0)) umma_commit_e(q_empty);      // all scores of the item have been issued
+          if (j == max(u1 - 2, u0)) umma_commit_e(&q_empty[x]);  // all scores of the item have been issued
           values(j);
           if (j + 2 < u1) scores(j + 2);
         }
@@ -431,36 +399,101 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
         cx += j1 - j0;
         had += j1 > j0;
       }
+    } else {
+      const int heads = p.head_pairs ? p.nh / 2 : p.nh;
+      const int BH = p.B * heads;
+      const int G = static_cast<int>(gridDim.x);
+      for (int it = 0;; ++it) {
+        const int w = it * G + ((it & 1) ? G - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
+        const bool more = w < n_items;       // an item past the end can only occur in a CTA's last round
+        mbar_wait(&i_empty[it & 1], ((it >> 1) & 1) ^ 1u, wctx, STATUS_TIMEOUT_PIPE_EMPTY);
+        FwdItem& item = items[it & 1];
+        if (more) {
+          const int bh = w % BH, b = bh / heads, h = bh % heads;
+          const size_t at = static_cast<size_t>(b) * n_levels + w / BH;
+          int row[2], j0[2], j1[2], hh[2], padded;
+          if (p.head_pairs) {
+            const int4 e = p.mask.plan_q[at];
+            hh[0] = 2 * h;
+            hh[1] = 2 * h + 1;
+            row[0] = row[1] = e.x * 128;
+            j0[0] = j0[1] = e.y >> 6;
+            j1[0] = j1[1] = max((e.z + 63) >> 6, j0[0] + 1);
+            padded = e.w;
+          } else {
+            const int4 e = p.mask.pairs[2 * at], f = p.mask.pairs[2 * at + 1];
+            hh[0] = hh[1] = h;
+            row[0] = e.x * 256;
+            row[1] = row[0] + 128;
+            j0[0] = e.y;
+            j1[0] = e.z;
+            j0[1] = e.w;
+            j1[1] = f.x;
+            padded = f.y;
+          }
+          const int *first = p.mask.first + static_cast<size_t>(b) * p.S_pad, *last = p.mask.last + static_cast<size_t>(b) * p.S_pad;
+          int lo[2][4], hi[2][4];
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int at_row = min(row[x], p.S_pad - 128) + 32 * i + lane;     // (no second tile: rows that nobody uses)
+              lo[x][i] = first[at_row];
+              hi[x][i] = last[at_row];
+            }
+          if (lane < 2) {
+            const int x = lane, a = min(x == 0 ? row[0] : row[1], p.S_pad - 128);
+            item.h[x] = x == 0 ? hh[0] : hh[1];
+            item.row[x] = x == 0 ? row[0] : row[1];
+            item.j0[x] = x == 0 ? j0[0] : j0[1];
+            item.j1[x] = x == 0 ? j1[0] : j1[1];
+            item.lo_max[x] = first[min(a + 127, p.S - 1)];
+            item.hi_min[x] = last[a];
+            item.slope2[x] = DIST ? -p.score.slopes[x == 0 ? hh[0] : hh[1]] * LOG2E_F : 0.f;
+            item.b = b;
+            item.padded = padded;
+          }
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              item.lo[x][32 * i + lane] = lo[x][i];
+              item.hi[x][32 * i + lane] = hi[x][i];
+            }
+        }
+        if (lane == 0) item.more = more;
+        __syncwarp();
+        mbar_arrive(&i_full[it & 1]);
+        if (!more || *abort_flag) break;
+        if (lane == 0) {
+          for (int x = 0; x < 2; ++x) {        // (rows past S: zeros)
+            mbar_wait(&q_empty[x], (it & 1) ^ 1u, wctx, STATUS_TIMEOUT_PIPE_EMPTY);  // the tile's score MMAs of the previous item are done
+            mbar_arrive_expect_tx(&q_full[x], Q_TILE);
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+              tma_load_4d(Qs + x * Q_TILE + db * 16384, &tq, &q_full[x], db * 64, item.row[x], item.h[x], item.b);
+          }
+        }
+        __syncwarp();
+      }
     }
   } else {
     setmaxnreg_inc<MFWD_REGS_SOFTMAX>();
-    const int x = (warp - MFWD_FIRST_SW) >> 2;   // query tile of this warp
+    const int x = (warp - MFWD_FIRST_SW) >> 2;         // query tile of this warp
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_base + x * 128;
     const uint32_t o_addr = tmem_base + lane_base + O_COL + x * D;
-    uint8_t* stage = staging + (warp - MFWD_FIRST_SW) * 4096;
+    uint8_t* stage = staging + (warp - MFWD_FIRST_SW) * 2048;
     constexpr bool MAXED = SCORES != BOUNDED;
     const float sl2 = p.score.sl2, cap2 = p.score.cap2;
     const float k = SCORES != PLAIN || DIST ? 1.f : sl2;    // what turns the numbers in the registers into exponents
     const uint64_t k_2 = pack_f32x2(k, k), sl2_2 = pack_f32x2(sl2, sl2);
     const uint64_t cap_2 = pack_f32x2(cap2, cap2), m2cap_2 = pack_f32x2(-2.f * cap2, -2.f * cap2);
-    // The ends of what a row sees, and what every row of the tile does.
     struct Rows {
       int lo, hi, lo_max, hi_min;
       float slope2;
-    };
-    auto rows_of = [&](const Item& i) {
-      Rows q;
-      const int *first = p.mask.first + static_cast<size_t>(i.b) * p.S_pad, *last = p.mask.last + static_cast<size_t>(i.b) * p.S_pad;
-      const int a = x == 0 ? i.row[0] : min(i.row[1], p.S_pad - 128);   // (no second tile: loads that nobody uses)
-      q.lo = first[a + r];
-      q.hi = last[a + r];
-      q.lo_max = first[min(a + 127, p.S - 1)];
-      q.hi_min = last[a];
-      q.slope2 = DIST ? -p.score.slopes[i.h[x]] * LOG2E_F : 0.f;
-      return q;
     };
     // 32 scores of a row from column col on -> exponents (plain ones: still to be scaled), dead ones -inf
     auto transform = [&](uint32_t (&v)[32], int col, const Rows& q, int row, bool whole) {
@@ -499,18 +532,12 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       }
     };
     int cdone = 0;  // blocks of this tile processed in earlier items
-    Walk walk = start();
-    Item item;
-    bool more = next(walk, item);
-    Rows rows = {};
-    if (more) rows = rows_of(item);
-    while (more) {
-      const Item cur = item;
-      const Rows q = rows;
-      more = next(walk, item);
-      if (more) rows = rows_of(item);           // on their way while this item is worked on
-      const int j0 = x == 0 ? cur.j0[0] : cur.j0[1], j1 = x == 0 ? cur.j1[0] : cur.j1[1];
-      const int row = (x == 0 ? cur.row[0] : cur.row[1]) + r;
+    for (int it = 0;; ++it) {
+      const FwdItem& item = item_of(it);
+      if (item.more == 0 || *abort_flag) break;
+      const Rows q{item.lo[x][r], item.hi[x][r], item.lo_max[x], item.hi_min[x], item.slope2[x]};
+      const int j0 = item.j0[x], j1 = item.j1[x], row = item.row[x] + r, b = item.b, h = item.h[x];
+      release_item(it);
       float m = MAXED ? -INFINITY : 0.f;
       uint64_t l2 = 0, t2 = 0;                  // sums of the probabilities, as they are and as rounded to bf16
       // 32 exponents -> probabilities, packed, and their sums
@@ -541,13 +568,15 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
         transform(v1, j * 64 + 32, q, row, whole);
         uint64_t moff2 = 0;
         if (MAXED) {
-          float mx0 = -INFINITY, mx1 = -INFINITY;
+          float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
+          for (int e = 0; e < 32; e += 4) {
             mx0 = fmax3(mx0, __uint_as_float(v0[e]), __uint_as_float(v0[e + 1]));
-            mx1 = fmax3(mx1, __uint_as_float(v1[e]), __uint_as_float(v1[e + 1]));
+            mx1 = fmax3(mx1, __uint_as_float(v0[e + 2]), __uint_as_float(v0[e + 3]));
+            mx2 = fmax3(mx2, __uint_as_float(v1[e]), __uint_as_float(v1[e + 1]));
+            mx3 = fmax3(mx3, __uint_as_float(v1[e + 2]), __uint_as_float(v1[e + 3]));
           }
-          const float m_new = fmaxf(m, fmaxf(mx0, mx1));
+          const float m_new = fmax3(m, fmaxf(mx0, mx1), fmaxf(mx2, mx3));
           // The running maximum is raised only when it grew by more than 2^8 (or was still -inf): raising it rescales the
           // accumulator in tensor memory, which after the first blocks is rare.
           bool grow = false;
@@ -601,34 +630,30 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
         // little but one key has that key's value exactly. The backward recomputes them unrounded and gets the other sum.
         const float2 lp = unpack_f32x2(l2), tp = unpack_f32x2(t2);
         const float l = lp.x + lp.y, t = tp.x + tp.y;
-        const float inv = q.lo < q.hi && t > 0.f ? 1.f / t : 0.f;
+        const bool seen = q.lo < q.hi;
+        const float inv = seen && t > 0.f ? 1.f / t : 0.f;
         const int c_last = cdone + j1 - j0 - 1;
         mbar_wait(&o_full[2 * x + (c_last & 1)], (c_last >> 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
         tc_fence_after();
         const int row0 = row - lane;
-        __nv_bfloat16* g0 = p.O + row0 * p.o_ss + cur.b * p.o_bs + (x == 0 ? cur.h[0] : cur.h[1]) * p.o_hs;
-        const bool seen = q.lo < q.hi;
+        __nv_bfloat16* g0 = p.O + row0 * p.o_ss + b * p.o_bs + h * p.o_hs;
 #pragma unroll
-        for (int hf = 0; hf < DB; ++hf) {
-          uint32_t wa[32], wb[32], ow[32];
-          tmem_ld_32x32(o_addr + hf * 64, wa);
-          tmem_ld_32x32(o_addr + hf * 64 + 32, wb);
-          tmem_ld_wait_for(wa);
-          tmem_ld_wait_for(wb);
-          if (hf == DB - 1) {        // the next item's first P V may overwrite the accumulator
+        for (int cc = 0; cc < D / 32; ++cc) {
+          uint32_t w[32], ow[16];
+          tmem_ld_32x32(o_addr + cc * 32, w);
+          tmem_ld_wait_for(w);
+          if (cc == D / 32 - 1) {    // the next item's first P V may overwrite the accumulator
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&o_empty[x]);
           }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            ow[e] = seen ? pack_bf16x2(__uint_as_float(wa[2 * e]) * inv, __uint_as_float(wa[2 * e + 1]) * inv) : 0u;
-            ow[16 + e] = seen ? pack_bf16x2(__uint_as_float(wb[2 * e]) * inv, __uint_as_float(wb[2 * e + 1]) * inv) : 0u;
-          }
-          store_rows_32x64(stage, ow, lane, g0 + hf * 64, p.o_ss, p.S - row0);
+          for (int e = 0; e < 16; ++e)
+            ow[e] = seen ? pack_bf16x2(__uint_as_float(w[2 * e]) * inv, __uint_as_float(w[2 * e + 1]) * inv) : 0u;
+          store_rows_32x32(stage, ow, lane, g0 + cc * 32, p.o_ss, p.S - row0);
         }
         if (p.lse != nullptr)
-          p.lse[(static_cast<size_t>(cur.b) * p.nh + (x == 0 ? cur.h[0] : cur.h[1])) * p.S_pad + row] =
+          p.lse[(static_cast<size_t>(b) * p.nh + h) * p.S_pad + row] =
               l > 0.f ? m * k + log2f(l) : (l == 0.f ? INFINITY : l);
       }
       cdone += j1 - j0;
