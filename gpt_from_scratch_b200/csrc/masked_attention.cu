@@ -83,6 +83,9 @@ __device__ __forceinline__ void sort_tiles(const int* lo, const int* hi, int S, 
   }
 }
 
+// N: tokens per thread and step. A scan costs the same for 1,024 tokens as for 8,192 (1 -> 8 a thread, us: one sequence of 8192
+// with a prefix 30 -> 12; up to 2,048 tokens one a thread is as fast, and loads and stores are contiguous).
+template <int N>
 __global__ void __launch_bounds__(MASK_THREADS) attention_mask_kernel(const MaskArgs a) {
   pdl_wait();
   pdl_trigger();
@@ -91,60 +94,171 @@ __global__ void __launch_bounds__(MASK_THREADS) attention_mask_kernel(const Mask
   const int b = blockIdx.x;
   const size_t row = static_cast<size_t>(b) * a.S;
   const size_t prow = static_cast<size_t>(b) * a.S_pad;
-  auto id_of = [&](int i) -> long long {
-    if (a.ids == nullptr) return 0;
-    return a.ids64 ? static_cast<const long long*>(a.ids)[row + i] : static_cast<const int*>(a.ids)[row + i];
+  const int chunks = (a.S_pad + MASK_THREADS * N - 1) / (MASK_THREADS * N);      // (S_pad < 2^31 - 2^13: S is checked)
+  // what a thread's tokens hold: the first of a document, prefix, padding (bits)
+  struct Tokens {
+    unsigned starts, prefix, pad;
   };
-  auto starts = [&](int i) { return i == 0 || id_of(i) != id_of(i - 1); };
-  const int chunks = (a.S + MASK_THREADS - 1) / MASK_THREADS;
-  // from the right: the end of the document, and the first token after this one that is not of the prefix's run
-  int carry = a.S, carry2 = a.S;
-  for (int c = chunks - 1; c >= 0; --c) {
-    const int i = c * MASK_THREADS + threadIdx.x;
-    const bool in = i < a.S;
-    const bool edge = in && starts(i);
+  // (all loads of a thread are issued before the first is looked at)
+  auto load = [&](int i0) {
+    Tokens t = {0u, 0u, 0u};
+    long long ids[N + 1] = {};
+    uint8_t pre[N] = {};
+    // whole vectors where rows of ids (prefix marks) begin at one: single elements of 1,024 threads, N apart, take N times the cycles
+    const bool wide = N % 4 == 0 && !a.ids64 && (a.S & 3) == 0 && (reinterpret_cast<uintptr_t>(a.ids) & 15) == 0 && i0 + N <= a.S;
+    const bool wide_p = N == 8 && (a.S & 7) == 0 && (reinterpret_cast<uintptr_t>(a.prefix) & 7) == 0 && i0 + N <= a.S;
+    if (a.ids != nullptr && wide) {
+      const int* from = static_cast<const int*>(a.ids) + row + i0;
+      if (i0 > 0) ids[0] = from[-1];
+#pragma unroll
+      for (int e = 0; e + 3 < N; e += 4) {
+        const int4 v = *reinterpret_cast<const int4*>(from + e);
+        ids[e + 1] = v.x;
+        ids[e + 2] = v.y;
+        ids[e + 3] = v.z;
+        ids[e + 4] = v.w;
+      }
+    } else if (a.ids != nullptr && a.ids64) {
+#pragma unroll
+      for (int e = -1; e < N; ++e)
+        if (i0 + e >= 0 && i0 + e < a.S) ids[e + 1] = static_cast<const long long*>(a.ids)[row + i0 + e];
+    } else if (a.ids != nullptr) {
+#pragma unroll
+      for (int e = -1; e < N; ++e)
+        if (i0 + e >= 0 && i0 + e < a.S) ids[e + 1] = static_cast<const int*>(a.ids)[row + i0 + e];
+    }
+    if (a.prefix != nullptr && wide_p) {
+      const uint2 v = *reinterpret_cast<const uint2*>(a.prefix + row + i0);
+#pragma unroll
+      for (int e = 0; e < N; ++e) pre[e] = static_cast<uint8_t>((e < 4 ? v.x : v.y) >> (8 * (e & 3)));
+    } else if (a.prefix != nullptr) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (i0 + e < a.S) pre[e] = a.prefix[row + i0 + e];
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const bool in = i0 + e < a.S;
+      if (in && (i0 + e == 0 || ids[e + 1] != ids[e])) t.starts |= 1u << e;
+      if (in && pre[e] != 0) t.prefix |= 1u << e;
+      if (in && ids[e + 1] < 0) t.pad |= 1u << e;
+    }
+    return t;
+  };
+  // first stop at or behind a thread's first token, S where there is none
+  auto first_of = [&](unsigned stops, int i0) { return stops ? i0 + __ffs(stops) - 1 : 0x7fffffff; };
+  auto last_of = [&](unsigned stops, int i0) { return stops ? i0 + 31 - __clz(stops) : -1; };
+  constexpr unsigned ALL = N == 32 ? 0xffffffffu : (1u << N) - 1u;
+  // N numbers of a thread from or to a row of [B, S_pad]
+  auto put = [&](int* to, int i0, const int (&v)[N]) {
+    if (i0 >= a.S_pad) return;
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+      for (int e = 0; e < N; e += 4) *reinterpret_cast<int4*>(to + prow + i0 + e) = make_int4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) to[prow + i0 + e] = v[e];
+    }
+  };
+  auto get = [&](const int* from, int i0, int (&v)[N]) {
+    if (i0 >= a.S_pad) return;
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+      for (int e = 0; e < N; e += 4) {
+        const int4 x = *reinterpret_cast<const int4*>(from + prow + i0 + e);
+        v[e] = x.x;
+        v[e + 1] = x.y;
+        v[e + 2] = x.z;
+        v[e + 3] = x.w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = from[prow + i0 + e];
+    }
+  };
+  // from the right: the end of the document, and the first token after this one that is not of the prefix's run. Of one chunk they stay
+  // in registers, of several they wait in qlast and last.
+  int carry = a.S, carry2 = a.S, any = 0;
+  int ends[N], reaches[N] = {};
+  auto from_right = [&](int i0, const Tokens& t) {
+    const unsigned live = i0 >= a.S ? 0u : (a.S - i0 >= N ? ALL : (1u << (a.S - i0)) - 1u);
+    const unsigned stops = t.starts | (~t.prefix & live);
     int end, reach = 0;
-    block_scan<true>(edge ? i : 0x7fffffff, carry, end, tmp);
-    if (a.prefix != nullptr) block_scan<true>(in && (edge || !a.prefix[row + i]) ? i : 0x7fffffff, carry2, reach, tmp);
-    if (in) {
-      a.qlast[prow + i] = end;
-      a.last[prow + i] = reach;
+    block_scan<true>(first_of(t.starts, i0), carry, end, tmp);
+    if (a.prefix != nullptr) block_scan<true>(first_of(stops, i0), carry2, reach, tmp);
+#pragma unroll
+    for (int e = N - 1; e >= 0; --e) {
+      ends[e] = end;
+      reaches[e] = reach;
+      if ((t.starts >> e) & 1u) end = i0 + e;
+      if ((stops >> e) & 1u) reach = i0 + e;
     }
-  }
-  carry = carry2 = -1;
-  int any = 0;
-  for (int c = 0; c < chunks; ++c) {
-    const int i = c * MASK_THREADS + threadIdx.x;
-    const bool in = i < a.S;
-    int before;
-    const int start = block_scan<false>(in && starts(i) ? i : -1, carry, before, tmp);
-    bool lead = false;
+  };
+  auto from_left = [&](int i0, const Tokens& t) {
+    int start, plain = -1;       // of the tokens before this thread's: the last start, the last token that is not prefix
+    block_scan<false>(last_of(t.starts, i0), carry, start, tmp);
     if (a.prefix != nullptr) {
-      const bool p = in && a.prefix[row + i];
-      const int plain = block_scan<false>(p ? -1 : i, carry2, before, tmp);   // the last token up to here that is not prefix
-      lead = p && plain < start;
+      const unsigned live = i0 >= a.S ? 0u : (a.S - i0 >= N ? ALL : (1u << (a.S - i0)) - 1u);
+      block_scan<false>(last_of(~t.prefix & live, i0), carry2, plain, tmp);
     }
-    if (in) {
-      const int end = a.qlast[prow + i];
-      int first = start, last = a.causal ? (lead ? a.last[prow + i] : i + 1) : end;
-      int qfirst = a.causal && !lead ? i : start, qlast = end;
+    if (t.pad != 0u) any = 1;
+    int out[4][N], place[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int i = i0 + e;
+      if ((t.starts >> e) & 1u) start = i;
+      const bool p = (t.prefix >> e) & 1u;
+      if (!p) plain = i;
+      const bool lead = p && plain < start;
+      int first = start, last = a.causal ? (lead ? reaches[e] : i + 1) : ends[e];
+      int qfirst = a.causal && !lead ? i : start, qlast = ends[e];
       if (a.window > 0) {
         first = max(first, i - a.window + 1);
         qlast = min(qlast, i + a.window);
       }
-      if (id_of(i) < 0) {
-        first = last = qfirst = qlast = i;      // wherever it does not widen a tile's range
-        any = 1;
-      }
-      a.first[prow + i] = first;
-      a.last[prow + i] = last;
-      a.qfirst[prow + i] = qfirst;
-      a.qlast[prow + i] = qlast;
-      a.positions[row + i] = i - start;
+      if ((t.pad >> e) & 1u) first = last = qfirst = qlast = i;      // wherever it does not widen a tile's range
+      if (i >= a.S) first = last = qfirst = qlast = a.S;
+      out[0][e] = first;
+      out[1][e] = last;
+      out[2][e] = qfirst;
+      out[3][e] = qlast;
+      place[e] = i - start;
+    }
+    put(a.first, i0, out[0]);
+    put(a.last, i0, out[1]);
+    put(a.qfirst, i0, out[2]);
+    put(a.qlast, i0, out[3]);
+    if (N % 4 == 0 && (a.S & 3) == 0 && i0 + N <= a.S) {
+#pragma unroll
+      for (int e = 0; e + 3 < N; e += 4)
+        *reinterpret_cast<int4*>(a.positions + row + i0 + e) = make_int4(place[e], place[e + 1], place[e + 2], place[e + 3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (i0 + e < a.S) a.positions[row + i0 + e] = place[e];
+    }
+  };
+  if (chunks == 1) {
+    const int i0 = threadIdx.x * N;
+    const Tokens t = load(i0);
+    from_right(i0, t);
+    carry = carry2 = -1;
+    from_left(i0, t);
+  } else {
+    for (int c = chunks - 1; c >= 0; --c) {
+      const int i0 = (c * MASK_THREADS + threadIdx.x) * N;
+      from_right(i0, load(i0));
+      put(a.qlast, i0, ends);
+      put(a.last, i0, reaches);
+    }
+    carry = carry2 = -1;
+    for (int c = 0; c < chunks; ++c) {
+      const int i0 = (c * MASK_THREADS + threadIdx.x) * N;
+      get(a.qlast, i0, ends);
+      get(a.last, i0, reaches);
+      from_left(i0, load(i0));
     }
   }
-  for (int i = a.S + threadIdx.x; i < a.S_pad; i += MASK_THREADS)
-    a.first[prow + i] = a.last[prow + i] = a.qfirst[prow + i] = a.qlast[prow + i] = a.S;
   any = __syncthreads_or(any);
   if (threadIdx.x == 0) a.padded[b] = any;
   const size_t tiles = static_cast<size_t>(b) * (a.S_pad / 128);
@@ -698,7 +812,7 @@ extern "C" {
 // aligned.
 int gfs_attention_mask(const void* ids, int ids64, const void* prefix, int B, int S, int causal, int window, void* out,
                        void* stream) {
-  if (S < 0 || B < 0 || window < 0 || (!causal && (window > 0 || prefix != nullptr)) || S > 0x7fffff00) return -1;
+  if (S < 0 || B < 0 || window < 0 || (!causal && (window > 0 || prefix != nullptr)) || S > 0x7fff0000) return -1;
   if (S == 0 || B == 0) return 0;
   if (reinterpret_cast<uintptr_t>(out) & 15) return -2;
   int* o = static_cast<int*>(out);
@@ -707,7 +821,8 @@ int gfs_attention_mask(const void* ids, int ids64, const void* prefix, int B, in
                    o + l.first, o + l.last, o + l.qfirst, o + l.qlast, o + l.padded, o + l.positions,
                    reinterpret_cast<int4*>(o + l.plan_q), reinterpret_cast<int4*>(o + l.plan_k),
                    reinterpret_cast<int4*>(o + l.pairs)};
-  gfs_host::launch_pdl(attention_mask_kernel, dim3(B), dim3(MASK_THREADS), 0, static_cast<cudaStream_t>(stream), a);
+  gfs_host::launch_pdl(S > 2 * MASK_THREADS ? attention_mask_kernel<8> : attention_mask_kernel<1>, dim3(B), dim3(MASK_THREADS), 0,
+                       static_cast<cudaStream_t>(stream), a);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 

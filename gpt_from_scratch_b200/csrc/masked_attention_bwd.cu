@@ -22,58 +22,68 @@ using gfs_host::strides_ok;
 namespace {
 
 // ---------------------------------------------------------------------------
-// Pre-pass: dvec[b, h, s] = sum_d dO * O, 0 for padding (whatever its dO holds) and for rows S .. S_pad. D / 8 threads
-// per row, 16-byte loads, rows in the memory order of O (heads or tokens fastest).
+// Pre-pass: dvec[b, h, s] = sum_d dO * O, 0 for padding (whatever its dO holds) and for rows S .. S_pad. Eight threads per row,
+// 16 bytes (head_dim 128: twice) of each tensor, four rows a thread with all loads issued first; rows in the memory order of O
+// (heads or tokens fastest), one division by a constant of the launch per row.
 // ---------------------------------------------------------------------------
 constexpr int DVEC_ROWS = 4;
-__global__ void __launch_bounds__(256)
-masked_dvec_kernel(const __nv_bfloat16* dO, const __nv_bfloat16* O, float* __restrict__ dvec, const int* first,
-                   const int* last, int S, int S_pad, int B, int nh, int D, long long do_ss, long long do_bs,
-                   long long do_hs, long long o_ss, long long o_bs, long long o_hs, int s_fastest) {
+struct DvecArgs {
+  const __nv_bfloat16 *dO, *O;
+  float* dvec;
+  const int *first, *last, *padded;
+  int S, S_pad, nh;
+  long long do_ss, do_bs, do_hs, o_ss, o_bs, o_hs;
+  unsigned inner;              // length of the faster index: S_pad (tokens) or nh (heads)
+  unsigned long long magic;    // floor(2^40 / inner) + 1: row / inner = row * magic >> 40 for row < 2^24, inner <= 2^16; or 0
+  int s_fastest;
+};
+template <int D>
+__global__ void __launch_bounds__(256) masked_dvec_kernel(const DvecArgs a) {
   pdl_wait();
   pdl_trigger();
-  const int tpr = D >> 3;                       // 8 or 16 threads per row
-  const int rows_per_pass = blockDim.x / tpr;
-  const int sub = threadIdx.x % tpr;
-  const unsigned total = static_cast<unsigned>(S_pad) * B * nh;
-  const unsigned row0 = blockIdx.x * static_cast<unsigned>(rows_per_pass * DVEC_ROWS) + threadIdx.x / tpr;
-  uint4 x[DVEC_ROWS], y[DVEC_ROWS];
+  constexpr int V = D / 64;                     // 16-byte vectors a thread
+  const int sub = threadIdx.x & 7, b = blockIdx.y;
+  const unsigned total = static_cast<unsigned>(a.S_pad) * a.nh;
+  const unsigned row0 = blockIdx.x * (32u * DVEC_ROWS) + (threadIdx.x >> 3);
+  const bool padded = a.padded[b] != 0;
+  uint4 x[DVEC_ROWS][V], y[DVEC_ROWS][V];
   unsigned at[DVEC_ROWS];
 #pragma unroll
   for (int i = 0; i < DVEC_ROWS; ++i) {
-    const unsigned row = row0 + i * rows_per_pass;
-    x[i] = y[i] = make_uint4(0, 0, 0, 0);
-    unsigned h, b, s;
-    if (s_fastest) {
-      s = row % S_pad;
-      const unsigned bh = row / S_pad;
-      h = bh % nh;
-      b = bh / nh;
-    } else {
-      h = row % nh;
-      const unsigned sb = row / nh;
-      b = sb % B;
-      s = sb / B;
-    }
-    at[i] = (b * nh + h) * S_pad + s;
-    if (row < total && s < static_cast<unsigned>(S) && first[b * S_pad + s] < last[b * S_pad + s]) {
-      x[i] = *reinterpret_cast<const uint4*>(dO + s * do_ss + b * do_bs + h * do_hs + sub * 8);
-      y[i] = *reinterpret_cast<const uint4*>(O + s * o_ss + b * o_bs + h * o_hs + sub * 8);
+    const unsigned row = row0 + 32u * i;
+    const unsigned outer = a.magic != 0 ? static_cast<unsigned>((row * a.magic) >> 40) : row / a.inner;
+    const unsigned rest = row - outer * a.inner;
+    const unsigned s = a.s_fastest ? rest : outer, h = a.s_fastest ? outer : rest;
+    at[i] = h * a.S_pad + s;
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[i][v] = y[i][v] = make_uint4(0, 0, 0, 0);
+    const size_t m = static_cast<size_t>(b) * a.S_pad + s;
+    if (row < total && s < static_cast<unsigned>(a.S) && (!padded || a.first[m] < a.last[m])) {
+      const __nv_bfloat16* px = a.dO + s * a.do_ss + b * a.do_bs + h * a.do_hs + sub * 8;
+      const __nv_bfloat16* py = a.O + s * a.o_ss + b * a.o_bs + h * a.o_hs + sub * 8;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        x[i][v] = *reinterpret_cast<const uint4*>(px + 64 * v);
+        y[i][v] = *reinterpret_cast<const uint4*>(py + 64 * v);
+      }
     }
   }
 #pragma unroll
   for (int i = 0; i < DVEC_ROWS; ++i) {
-    const unsigned row = row0 + i * rows_per_pass;
-    const uint32_t xw[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-    const uint32_t yw[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
     float acc = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 a2 = unpack_bf16x2(xw[e]), b2 = unpack_bf16x2(yw[e]);
-      acc += a2.x * b2.x + a2.y * b2.y;
+    for (int v = 0; v < V; ++v) {
+      const uint32_t xw[4] = {x[i][v].x, x[i][v].y, x[i][v].z, x[i][v].w};
+      const uint32_t yw[4] = {y[i][v].x, y[i][v].y, y[i][v].z, y[i][v].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 a2 = unpack_bf16x2(xw[e]), b2 = unpack_bf16x2(yw[e]);
+        acc += a2.x * b2.x + a2.y * b2.y;
+      }
     }
-    for (int o = tpr >> 1; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    if (row < total && sub == 0) dvec[at[i]] = acc;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    if (row0 + 32u * i < total && sub == 0) a.dvec[static_cast<size_t>(b) * a.nh * a.S_pad + at[i]] = acc;
   }
 }
 
@@ -617,20 +627,21 @@ int gfs_masked_attention_bwd(const void* q, const void* k, const void* v, const 
     return -2;
   if (S <= 0 || B <= 0 || nh <= 0) return 0;
   const int S_pad = (S + 127) / 128 * 128;
-  if (static_cast<long long>(S_pad) * B * nh > 0x3fffffffll) return -1;   // 32-bit row numbers in the pre-pass
+  if (static_cast<long long>(S_pad) * nh > 0x3fffffffll || B > 65535) return -1;   // 32-bit row numbers in the pre-pass
+  if (static_cast<long long>(S_pad / 128) * B * nh > 0x7fffffffll) return -1;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const long long *sq = strides, *sk = strides + 3, *sv = strides + 6, *so = strides + 9, *sdo = strides + 12,
                   *sdq = strides + 15, *sdk = strides + 18, *sdv = strides + 21;
   MaskedBwdParams p = {};
   p.mask = mask_view(mask, B, S);
   {
-    const long long rows = static_cast<long long>(S_pad) * B * nh;
-    const int threads = 256;
-    const int rows_per_block = threads / (D >> 3) * DVEC_ROWS;
-    const dim3 grid(static_cast<unsigned>((rows + rows_per_block - 1) / rows_per_block));
-    gfs_host::launch_pdl(masked_dvec_kernel, grid, dim3(threads), 0, stream, static_cast<const __nv_bfloat16*>(dout),
-                         static_cast<const __nv_bfloat16*>(out), static_cast<float*>(dvec), p.mask.first, p.mask.last, S,
-                         S_pad, B, nh, D, sdo[0], sdo[1], sdo[2], so[0], so[1], so[2], so[0] < so[2] ? 1 : 0);
+    const int s_fastest = so[0] < so[2] ? 1 : 0;
+    const unsigned inner = s_fastest ? S_pad : nh, rows = static_cast<unsigned>(S_pad) * nh;
+    const DvecArgs a{static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out), static_cast<float*>(dvec),
+                     p.mask.first, p.mask.last, p.mask.padded, S, S_pad, nh, sdo[0], sdo[1], sdo[2], so[0], so[1], so[2], inner,
+                     rows + 32 * DVEC_ROWS < (1u << 24) && inner <= (1u << 16) ? (1ull << 40) / inner + 1 : 0ull, s_fastest};
+    const dim3 grid((rows + 32 * DVEC_ROWS - 1) / (32 * DVEC_ROWS), B);
+    gfs_host::launch_pdl(D == 64 ? masked_dvec_kernel<64> : masked_dvec_kernel<128>, grid, dim3(256), 0, stream, a);
     if (cudaGetLastError() != cudaSuccess) return -11;
   }
   const BwdMaps maps{make_map(q, D, S, nh, B, sq, 128), make_map(k, D, S, nkv, B, sk, 128),
