@@ -56,19 +56,41 @@ __device__ __forceinline__ Vec8<T> load_vec(const T* p) {
     reinterpret_cast<uint4*>(&r)[i] = reinterpret_cast<const uint4*>(p)[i];
   return r;
 }
+// pairs of 16-bit numbers at a time: one conversion instruction for two
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi, __nv_bfloat16) { return pack_bf16x2(lo, hi); }
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi, __half) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_pair(uint32_t u, __nv_bfloat16) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack_pair(uint32_t u, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 template <typename T>
 __device__ __forceinline__ void store_vec(T* p, const float (&f)[8]) {
-  Vec8<T> r;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) r.v[e] = from_f32<T>(f[e]);
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(Vec8<T>) / 16); ++i)
-    reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(&r)[i];
+  if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_pair(f[0], f[1], T()), pack_pair(f[2], f[3], T()), pack_pair(f[4], f[5], T()),
+                                              pack_pair(f[6], f[7], T()));
+  } else {
+    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+  }
 }
 template <typename T>
 __device__ __forceinline__ void to_floats(const Vec8<T>& x, float (&f)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    const uint4 u = *reinterpret_cast<const uint4*>(&x);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = to_f32(x.v[e]);
+    for (int e = 0; e < 4; ++e) {
+      const float2 v = unpack_pair(w[e], T());
+      f[2 * e] = v.x;
+      f[2 * e + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = to_f32(x.v[e]);
+  }
 }
 
 // A tensor [S, B, heads, D], its dimensions contiguous.
@@ -89,7 +111,7 @@ struct RotaryArgs {
   int pos64, rows;
   int S, B, n1, n2, n3, D, R;
   int inverse;            // rotate the other way
-  float eps;
+  float eps, inv_D;
   uint32_t* status;
 };
 
@@ -232,7 +254,7 @@ rotary_kernel(const RotaryArgs a, unsigned n_items, unsigned items_per_token, in
       to_pairs(f, v);
 #pragma unroll
       for (int e = 0; e < 4; ++e) ss = fma_f32x2(v[e], v[e], ss);
-      const float rstd = rsqrtf(group_sum<LANES>(pair_sum(ss)) / static_cast<float>(a.D) + a.eps);
+      const float rstd = rsqrtf(group_sum<LANES>(pair_sum(ss)) * a.inv_D + a.eps);
       const uint64_t r2 = pack_f32x2(rstd, rstd);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -259,7 +281,6 @@ qk_norm_rope_bwd_kernel(const RotaryArgs a, unsigned n_items, unsigned items_per
   const int group = (threadIdx.x & 31) / LANES;
   const int e0 = (threadIdx.x & (LANES - 1)) * 8;
   const bool lane_on = e0 < a.D;
-  const float inv_D = 1.f / static_cast<float>(a.D);
   uint64_t dw1[4] = {}, dw2[4] = {};
   for (unsigned item = blockIdx.x * ROT_WARPS + (threadIdx.x >> 5); item < n_items; item += gridDim.x * ROT_WARPS) {
     const unsigned token = item / items_per_token;
@@ -316,8 +337,8 @@ qk_norm_rope_bwd_kernel(const RotaryArgs a, unsigned n_items, unsigned items_per
           ss = fma_f32x2(v[e], v[e], ss);
           dot = fma_f32x2(zw[e], v[e], dot);
         }
-        const float rstd = rsqrtf(group_sum<LANES>(pair_sum(ss)) * inv_D + a.eps);
-        const float m = group_sum<LANES>(pair_sum(dot)) * rstd * rstd * inv_D;      // mean(dz w n) rstd
+        const float rstd = rsqrtf(group_sum<LANES>(pair_sum(ss)) * a.inv_D + a.eps);
+        const float m = group_sum<LANES>(pair_sum(dot)) * rstd * rstd * a.inv_D;      // mean(dz w n) rstd
         const uint64_t r2 = pack_f32x2(rstd, rstd), m2 = pack_f32x2(-m, -m);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -396,7 +417,7 @@ rotary_any_kernel(const RotaryArgs a, unsigned n_rows) {
     if (NORM) {
       float ss = 0.f;
       for (int d = lane; d < a.D; d += 32) ss += to_f32(x[d]) * to_f32(x[d]);
-      rstd = rsqrtf(warp_sum(ss) / static_cast<float>(a.D) + a.eps);
+      rstd = rsqrtf(warp_sum(ss) * a.inv_D + a.eps);
     }
     auto z = [&](int d) { return NORM ? to_f32(x[d]) * (rstd * to_f32(w[d])) : to_f32(x[d]); };
     for (int d = lane; d < a.D; d += 32)
@@ -446,8 +467,8 @@ qk_norm_rope_bwd_any_kernel(const RotaryArgs a, unsigned n_rows) {
     }
     float rstd = 1.f, m = 0.f;
     if (NORM) {
-      rstd = rsqrtf(warp_sum(ss) / static_cast<float>(a.D) + a.eps);
-      m = warp_sum(dot) * rstd * rstd / static_cast<float>(a.D);
+      rstd = rsqrtf(warp_sum(ss) * a.inv_D + a.eps);
+      m = warp_sum(dot) * rstd * rstd * a.inv_D;
     }
 #pragma unroll
     for (int i = 0; i < ROT_STEPS; ++i) {
@@ -643,7 +664,7 @@ int gfs_qk_norm_rope_fwd(const void* x, const long long* strides, const void* w1
   a.cos = static_cast<const float*>(cosb);
   a.sin = static_cast<const float*>(sinb);
   a.positions = positions; a.pos64 = pos64; a.rows = rows;
-  a.S = S; a.B = B; a.n1 = n1; a.n2 = n2; a.D = D; a.R = R; a.eps = eps;
+  a.S = S; a.B = B; a.n1 = n1; a.n2 = n2; a.D = D; a.R = R; a.eps = eps; a.inv_D = 1.f / D;
   a.status = gfs_host::status_words();
   return dispatch_type(a, dtype, half, w1 != nullptr, false, nullptr, nullptr, static_cast<cudaStream_t>(stream));
 }
@@ -670,7 +691,7 @@ int gfs_qk_norm_rope_bwd(const void* x, const void* dq, const void* dk, const vo
   a.cos = static_cast<const float*>(cosb);
   a.sin = static_cast<const float*>(sinb);
   a.positions = positions; a.pos64 = pos64; a.rows = rows;
-  a.S = S; a.B = B; a.n1 = n1; a.n2 = n2; a.n3 = n2; a.D = D; a.R = R; a.inverse = 1; a.eps = eps;
+  a.S = S; a.B = B; a.n1 = n1; a.n2 = n2; a.n3 = n2; a.D = D; a.R = R; a.inverse = 1; a.eps = eps; a.inv_D = 1.f / D;
   a.status = gfs_host::status_words();
   return dispatch_type(a, dtype, half, w1 != nullptr, true, dw1, dw2, static_cast<cudaStream_t>(stream));
 }
