@@ -609,7 +609,13 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       int lo, hi, lo_max, hi_min;
       float slope2;
     };
+    // bits [lo - col, hi - col) of 32: what the row sees
+    auto live_bits = [](const Rows& q, int col) {
+      const int a = max(q.lo - col, 0), z = q.hi - col;
+      return (z >= 32 ? 0xffffffffu : (z <= 0 ? 0u : (1u << z) - 1u)) & (a >= 32 ? 0u : 0xffffffffu << a);
+    };
     // 32 scores of a row from column col on -> exponents (plain ones: still to be scaled), dead ones -inf
+    // (bounded ones: dead probabilities become 0 afterwards)
     auto transform = [&](uint32_t (&v)[32], int col, const Rows& q, int row, bool whole) {
       if (SCORES != PLAIN || DIST) {
         const uint64_t slope_2 = pack_f32x2(q.slope2, q.slope2);
@@ -637,10 +643,8 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
           }
         }
       }
-      if (!whole) {
-        // bits [lo - col, hi - col) of 32
-        const int a = max(q.lo - col, 0), z = q.hi - col;
-        const uint32_t live = (z >= 32 ? 0xffffffffu : (z <= 0 ? 0u : (1u << z) - 1u)) & (a >= 32 ? 0u : 0xffffffffu << a);
+      if (MAXED && !whole) {
+        const uint32_t live = live_bits(q, col);
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = (live >> e) & 1u ? v[e] : 0xff800000u;
       }
@@ -655,14 +659,18 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       float m = MAXED ? -INFINITY : 0.f;
       uint64_t l2 = 0, t2 = 0;                  // sums of the probabilities, as they are and as rounded to bf16
       // 32 exponents -> probabilities, packed, and their sums
-      auto probabilities = [&](const uint32_t (&v)[32], uint32_t (&packed)[16], uint64_t moff2) {
+      auto probabilities = [&](const uint32_t (&v)[32], uint32_t (&packed)[16], uint64_t moff2, uint32_t live) {
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          const float2 y = MAXED ? unpack_f32x2(fma_f32x2(pack_u32x2(v[e], v[e + 1]), k_2, moff2))
-                                 : make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-          const float p0 = fast_exp2(y.x), p1 = fast_exp2(y.y);
-          const uint32_t w = pack_bf16x2(p0, p1);
-          l2 = add_f32x2(l2, pack_f32x2(p0, p1));
+          const uint64_t y2 = MAXED ? fma_f32x2(pack_u32x2(v[e], v[e + 1]), k_2, moff2) : pack_u32x2(v[e], v[e + 1]);
+          const float2 y = unpack_f32x2(y2);
+          float2 pr = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+          if (!MAXED && live != 0xffffffffu) {
+            pr.x = (live >> e) & 1u ? pr.x : 0.f;
+            pr.y = (live >> (e + 1)) & 1u ? pr.y : 0.f;
+          }
+          const uint32_t w = pack_bf16x2(pr.x, pr.y);
+          l2 = add_f32x2(l2, pack_f32x2(pr.x, pr.y));
           t2 = add_f32x2(t2, pack_u32x2(w << 16, w & 0xffff0000u));
           packed[e >> 1] = w;
         }
@@ -730,9 +738,9 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
           moff2 = pack_f32x2(-moff, -moff);
         }
         // the probabilities go where the scores were: all of those are in registers
-        probabilities(v0, pk, moff2);
+        probabilities(v0, pk, moff2, MAXED || whole ? 0xffffffffu : live_bits(q, j * 64));
         tmem_st_32x16(at, pk);
-        probabilities(v1, pk, moff2);
+        probabilities(v1, pk, moff2, MAXED || whole ? 0xffffffffu : live_bits(q, j * 64 + 32));
         tmem_st_32x16(at + 16, pk);
         tmem_st_wait();
         tc_fence_before();

@@ -95,7 +95,7 @@ def document_ids(B, S, kind, seed):
     return torch.tensor(rows, device="cuda")
 
 
-@pytest.mark.parametrize("B,S", [(1, 1), (3, 2), (2, 127), (2, 128), (1, 129), (2, 1023), (2, 1025), (1, 5000)])
+@pytest.mark.parametrize("B,S", [(1, 1), (3, 2), (2, 127), (2, 128), (1, 129), (2, 1023), (2, 1025), (1, 2304), (1, 5001), (2, 17003)])
 @pytest.mark.parametrize("kind", ["none", "docs", "padded", "empty"])
 def test_mask(cuda_device, B, S, kind):
     ids = document_ids(B, S, kind, S)
@@ -118,11 +118,19 @@ def test_mask(cuda_device, B, S, kind):
             mask.buffer[layout[name]:layout[name] + math.prod(shape)].view(shape).cpu()
             for name, shape in (("qfirst", (B, S_pad)), ("qlast", (B, S_pad)), ("padded", (B,)), ("plan_q", (B, tiles, 4)),
                                 ("plan_k", (B, tiles, 4))))
-        see = cpu.visible()
-        j_any = see.any(1)
-        rows = torch.arange(S)[None, :, None]
-        lo = torch.where(see, rows, S).amin(1)
-        hi = torch.where(see, rows + 1, 0).amax(1)
+        # (by their first and last: both ends grow, so a query sees j from the first whose last is past j to the last whose first is not)
+        at = torch.arange(S).expand(B, S).contiguous()
+        lo = torch.searchsorted(cpu.last.long().contiguous(), at, right=True)
+        hi = torch.searchsorted(cpu.first.long().contiguous(), at, right=True)
+        j_any = torch.zeros(B, S, dtype=torch.bool) | (ids >= 0).cpu() if ids is not None else torch.ones(B, S, dtype=torch.bool)
+        # queries that are padding see nothing and may lie in front of the first or behind the last
+        if S <= 2500:
+            see = cpu.visible()
+            rows = torch.arange(S)[None, :, None]
+            assert torch.equal(j_any, see.any(1))
+            lo, hi = torch.where(see, rows, S).amin(1), torch.where(see, rows + 1, 0).amax(1)
+        elif kind in ("padded", "empty"):
+            lo, hi = qfirst[:, :S], qlast[:, :S]
         assert torch.equal(torch.where(j_any, qfirst[:, :S], 0), torch.where(j_any, lo, 0).int())
         assert torch.equal(torch.where(j_any, qlast[:, :S], 0), torch.where(j_any, hi, 0).int())
         assert (qfirst[:, :S][~j_any] == qlast[:, :S][~j_any]).all() and (qfirst[:, S:] == S).all() and (qlast[:, S:] == S).all()
