@@ -5,6 +5,8 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
+from .ops.rope import RopeScaling
+
 
 @dataclass
 class GPTConfig:
@@ -22,6 +24,12 @@ class GPTConfig:
     init_method: str = "xavier_uniform"   # or "normal"
     init_std: float = 0.02
     attention_impl: str = "fused"         # "fused": tcgen05 flash attention on CUDA; "torch": eager oracle
+    rope_scaling: RopeScaling | None = None  # angles for contexts longer than trained on (ops/rope.py)
+    # Any of these four sends attention through ops/qk_norm_rope.py and ops/masked_attention.py:
+    qk_norm: bool = False                 # RMSNorm of every head of q and k, before the rotation
+    attention_softcap: float = 0.0        # c > 0: scores become c tanh(score / c)
+    attention_window: int = 0             # w > 0: no token sees one more than w - 1 before it
+    eod_token_id: int = -1                # >= 0: documents end with it, tokens see (and count positions in) their own only
     reference_quirks: bool = False        # reproduce reference behaviours that were fixed by default
 
     def flops_per_token(self, seq_len: int) -> float:
@@ -31,4 +39,5 @@ class GPTConfig:
 
     def num_parameters(self) -> int:
         H, I, L, V = self.hidden_size, self.intermediate_size, self.num_layers, self.vocab_size
-        return 2 * V * H + L * (4 * H * H + 3 * H * I + 2 * H) + H
+        qk = 2 * (H // self.num_attention_heads) if self.qk_norm else 0
+        return 2 * V * H + L * (4 * H * H + 3 * H * I + 2 * H + qk) + H

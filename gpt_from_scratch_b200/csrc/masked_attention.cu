@@ -406,9 +406,9 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
 
   // Items: the widest first, dealt to the CTAs in a snake; all barrier parities run on counters that continue across items.
   // What a warp wants of the it-th item it copies out of its slot, then it releases the slot.
-  auto item_of = [&](int it) -> const FwdItem& {
+  auto take_item = [&](int it) {        // false, for the whole warp: there are no more, or a wait has given up
     mbar_wait(&i_full[it & 1], (it >> 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
-    return items[it & 1];
+    return !__any_sync(0xffffffffu, items[it & 1].more == 0 || *abort_flag != 0);
   };
   auto release_item = [&](int it) {
     __syncwarp();
@@ -425,9 +425,8 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
     setmaxnreg_dec<MFWD_REGS_IO>();
     if (warp == 0) {
       int g = 0;      // key blocks loaded so far (ring position)
-      for (int it = 0;; ++it) {
-        const FwdItem& item = item_of(it);
-        if (item.more == 0 || *abort_flag) break;
+      for (int it = 0; take_item(it); ++it) {
+        const FwdItem& item = items[it & 1];
         const int bb = item.b, kvh = item.h[0] / p.group;
         const Blocks u = blocks_of(item);
         release_item(it);
@@ -463,9 +462,8 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       int g0 = 0;               // ring position of this item's first key block
       int cx = 0;               // this tile's blocks in earlier items (barrier phases)
       int had = 0;              // items in which it had blocks (phase of o_empty)
-      for (int it = 0;; ++it) {
-        const FwdItem& item = item_of(it);
-        if (item.more == 0 || *abort_flag) break;
+      for (int it = 0; take_item(it); ++it) {
+        const FwdItem& item = items[it & 1];
         const int u0 = blocks_of(item).u0, u1 = blocks_of(item).u1;
         const int j0 = item.j0[x], j1 = item.j1[x];
         const bool padded = item.padded != 0;
@@ -578,7 +576,7 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
         if (lane == 0) item.more = more;
         __syncwarp();
         mbar_arrive(&i_full[it & 1]);
-        if (!more || *abort_flag) break;
+        if (!more || __any_sync(0xffffffffu, *abort_flag != 0)) break;
         if (lane == 0) {
           for (int x = 0; x < 2; ++x) {        // (rows past S: zeros)
             mbar_wait(&q_empty[x], (it & 1) ^ 1u, wctx, STATUS_TIMEOUT_PIPE_EMPTY);  // the tile's score MMAs of the previous item are done
@@ -590,6 +588,7 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
         }
         __syncwarp();
       }
+      if (lane == 0) settle_copies(wctx);
     }
   } else {
     setmaxnreg_inc<MFWD_REGS_SOFTMAX>();
@@ -650,9 +649,8 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       }
     };
     int cdone = 0;  // blocks of this tile processed in earlier items
-    for (int it = 0;; ++it) {
-      const FwdItem& item = item_of(it);
-      if (item.more == 0 || *abort_flag) break;
+    for (int it = 0; take_item(it); ++it) {
+      const FwdItem& item = items[it & 1];
       const Rows q{item.lo[x][r], item.hi[x][r], item.lo_max[x], item.hi_min[x], item.slope2[x]};
       const int j0 = item.j0[x], j1 = item.j1[x], row = item.row[x] + r, b = item.b, h = item.h[x];
       release_item(it);

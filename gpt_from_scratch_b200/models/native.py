@@ -146,6 +146,7 @@ class _Plan:
             a, m = child(layer, "attention", ParallelAttention), child(layer, "mlp", ParallelMLP)
             nh, D = read(a.__dict__, "num_heads_per_partition"), read(a.__dict__, "head_dim")
             _require(read(a.__dict__, "attention_impl") == "fused" and D in (64, 128) and nh * D == H)
+            _require(read(a.__dict__, "masked") is False)       # masked attention is the modules'
             ws = (w1, linear(a, "qkv_proj", ColumnParallelLinear, 3 * H, H),
                   linear(a, "out_proj", RowParallelLinear, H, H), w2,
                   linear(m, "gate_up_proj", ColumnParallelLinear), linear(m, "down_proj", RowParallelLinear))

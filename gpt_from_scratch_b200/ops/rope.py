@@ -142,7 +142,8 @@ def rows_of(t: torch.Tensor) -> torch.Tensor:
 def check_tables(what: str, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None,
                  S: int, B: int, D: int) -> int:
     """Checks the arguments that all rotations share; returns the number of rotated dimensions."""
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+    table_type = torch.float64 if cos.dtype == x.dtype == torch.float64 else torch.float32
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != table_type or sin.dtype != table_type:
         raise ValueError(f"{what}: cos and sin have to be fp32 tables of one shape [positions, rotary_dim / 2]")
     R = 2 * cos.shape[1]
     if not 0 < R <= D:

@@ -16,6 +16,7 @@ import torch.distributed as dist
 
 from gpt_from_scratch_b200.checkpoint import latest_step, load_checkpoint, save_checkpoint
 from gpt_from_scratch_b200.config import GPTConfig
+from gpt_from_scratch_b200.ops.rope import RopeScaling
 from gpt_from_scratch_b200.data import PrefetchLoader, create_distributed_dataloader, write_synthetic_tokens
 from gpt_from_scratch_b200.engine import TrainEngine
 from gpt_from_scratch_b200.parallel import parallel_state as ps
@@ -52,6 +53,15 @@ def parse_args(argv=None):
     p.add_argument("--backend", choices=["nccl", "gloo"], default=None)
     p.add_argument("--device", choices=["cuda", "cpu"], default=None)
     p.add_argument("--attention-impl", choices=["fused", "torch"], default="fused")
+    p.add_argument("--qk-norm", action="store_true", help="RMSNorm of every head of q and k")
+    p.add_argument("--attention-softcap", type=float, default=0.0, help="c > 0: attention scores become c tanh(score / c)")
+    p.add_argument("--attention-window", type=int, default=0, help="w > 0: no token sees one more than w - 1 before it")
+    p.add_argument("--eod-token-id", type=int, default=-1,
+                   help="id >= 0 that ends a document: tokens see only their own document")
+    p.add_argument("--rope-scaling", choices=["linear", "ntk", "by_parts"], default=None,
+                   help="rotary angles for contexts longer than trained on (ops/rope.py: RopeScaling)")
+    p.add_argument("--rope-scaling-factor", type=float, default=1.0)
+    p.add_argument("--rope-original-length", type=int, default=0, help="context that by_parts scaling starts from")
     p.add_argument("--comm-impl", choices=["fused", "nccl"], default="nccl",
                    help="fused: peer-memory kernels that overlap the collective with the GEMM")
     p.add_argument("--cuda-graph", action="store_true",
@@ -80,7 +90,11 @@ def build_config(args) -> GPTConfig:
         max_position_embeddings=max(args.max_position_embeddings, args.seq_len),
         intermediate_size=args.intermediate_size, rms_norm_eps=args.rms_norm_eps,
         dropout_prob=args.dropout_prob, init_method=args.init_method, init_std=args.init_std,
-        attention_impl=args.attention_impl, reference_quirks=args.reference_quirks)
+        attention_impl=args.attention_impl, reference_quirks=args.reference_quirks,
+        rope_scaling=RopeScaling(args.rope_scaling, args.rope_scaling_factor, args.rope_original_length)
+        if args.rope_scaling else None,
+        qk_norm=args.qk_norm, attention_softcap=args.attention_softcap, attention_window=args.attention_window,
+        eod_token_id=args.eod_token_id)
 
 
 def init_distributed(args):
