@@ -107,8 +107,20 @@ struct MaskedBwdParams {
 };
 
 constexpr int MBWD_CW = 16;                         // compute warps
-constexpr int MBWD_FIRST_CW = 4;                    // warps 0-2: TMA, score MMAs, gradient MMAs; 3: idle
+constexpr int MBWD_FIRST_CW = 4;                    // warps 0-2: TMA, score MMAs, gradient MMAs; 3: items
 constexpr int MBWD_THREADS = 32 * (MBWD_FIRST_CW + MBWD_CW);
+
+// A work item, as warp 3 puts it into shared memory one ahead of the others: nobody else divides or waits for the plans. At
+// head_dim 64 there is room for what the resident rows see and (mode 1) their statistics too.
+struct alignas(16) BwdItem {
+  int more;                    // 0: there are no further items
+  int b, h, rt, part, padded;
+  int t_begin, n_t;            // streamed tiles per head (at least one, which may be masked whole)
+};
+struct BwdRows {
+  int lo[128], hi[128];
+  float lse[128], dvec[128];
+};
 
 template <int D, int MODE>
 struct MBwdShape {
@@ -117,7 +129,9 @@ struct MBwdShape {
   static constexpr int TS = D == 64 ? 7 : 4;
   static constexpr int STAGE_BYTES = 2048;          // per compute warp, to transpose its output rows through
   static constexpr int STAGING = MBWD_CW * STAGE_BYTES;
-  static constexpr int SMEM = 2 * (D / 64) * 16384 + 2 * TS * (D / 64) * 8192 + STAGING + (MODE == 0 ? TS * 512 : 0) + 256;
+  static constexpr bool ROWS = D == 64;             // BwdRows beside the items
+  static constexpr int ITEMS = 2 * static_cast<int>(sizeof(BwdItem) + (ROWS ? sizeof(BwdRows) : 0));
+  static constexpr int SMEM = 2 * (D / 64) * 16384 + 2 * TS * (D / 64) * 8192 + STAGING + (MODE == 0 ? TS * 512 : 0) + ITEMS + 256;
 };
 
 // Sixteen compute warps: two groups of eight take alternate streamed tiles (group = X/Y buffer); within a group two warps
@@ -147,7 +161,9 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
   uint8_t* T2 = T1 + TS * T_BYTES;
   uint8_t* staging = T2 + TS * T_BYTES;
   float* stats = reinterpret_cast<float*>(staging + Shape::STAGING);  // mode 0: [TS stages][lse 64 | dvec 64]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(stats) + (MODE == 0 ? TS * 512 : 0));
+  BwdItem* items = reinterpret_cast<BwdItem*>(reinterpret_cast<uint8_t*>(stats) + (MODE == 0 ? TS * 512 : 0));   // [2]
+  BwdRows* item_rows = reinterpret_cast<BwdRows*>(items + 2);                                                 // [2]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(items) + Shape::ITEMS);
   uint64_t* r_full = bars;
   uint64_t* t_full = bars + 1;             // [TS]
   uint64_t* t_empty = t_full + TS;         // [TS]
@@ -158,7 +174,9 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
   uint64_t* acc_full = m_empty + 2;
   uint64_t* acc_empty = acc_full + 1;
   uint64_t* r_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 3);
+  uint64_t* i_full = acc_full + 3;         // [2]
+  uint64_t* i_empty = i_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(i_empty + 2);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -167,57 +185,13 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     if (threadIdx.x == 0) record_status(p.status, STATUS_BAD_ARGUMENT, 0x5a23u);
     return;
   }
-  const int heads = MODE == 0 ? p.nh / p.group : p.nh;
-  const int BHP = p.B * heads * p.parts;
   // the rows that a resident row sees: queries of a key, keys of a query
   const int* const lo_all = MODE == 0 ? p.mask.qfirst : p.mask.first;
   const int* const hi_all = MODE == 0 ? p.mask.qlast : p.mask.last;
   // Persistent: a CTA walks work items (resident tile, batch * head * part), the heaviest first, dealt in a snake over the
   // CTAs; barrier phases run on counters that continue across items, so the next item's loads and first score MMAs overlap
   // this one's epilogue.
-  const int G = static_cast<int>(gridDim.x);
   const int hpi = MODE == 0 ? p.group / p.parts : 1;    // heads per item
-  const int4* const plans = MODE == 0 ? p.mask.plan_k : p.mask.plan_q;
-  struct Item {
-    int rt, b, h, part, t_begin, n_t;    // n_t: streamed tiles per head (at least one, which may be masked whole)
-  };
-  struct Walk {                          // the items of this CTA, the next one's plan already on its way
-    int it, w;
-    int4 plan;
-  };
-  auto where = [&](int it) { return it * G + ((it & 1) ? G - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x)); };
-  auto split = [&](int w, int& b, int& h, int& part) {
-    int r = w % BHP;
-    part = r % p.parts;
-    r /= p.parts;
-    h = r % heads;
-    b = r / heads;
-  };
-  auto fetch = [&](Walk& k) {
-    k.w = where(k.it);
-    if (k.w < n_items) {
-      int b, h, part;
-      split(k.w, b, h, part);
-      k.plan = plans[static_cast<size_t>(b) * n_rt + k.w / BHP];
-    }
-  };
-  auto start = [&]() {
-    Walk k;
-    k.it = 0;
-    fetch(k);
-    return k;
-  };
-  // the next item, or false: an item past the end can only occur in a CTA's last round
-  auto next = [&](Walk& k, Item& i) {
-    if (k.w >= n_items) return false;
-    split(k.w, i.b, i.h, i.part);
-    i.rt = k.plan.x;
-    i.t_begin = k.plan.y >> 6;
-    i.n_t = max(((k.plan.z + 63) >> 6) - i.t_begin, 1);
-    ++k.it;
-    fetch(k);
-    return true;
-  };
 
   if (threadIdx.x == 0) {
     mbar_init(r_full, 1);
@@ -234,6 +208,10 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, EPI_WARPS);
     mbar_init(r_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&i_full[i], 32);
+      mbar_init(&i_empty[i], 3 + MBWD_CW);
+    }
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tr1);
@@ -255,13 +233,25 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
   pdl_trigger();
   const uint32_t tmem_base = *tmem_slot;
   WaitCtx wctx{abort_flag, p.status, GFS_WAIT_LIMIT_NS};
+  // The it-th item is copied out of its slot and the slot released; false, for the whole warp: there are no more, or a wait has
+  // given up.
+  auto take_item = [&](int it, BwdItem& item) {
+    mbar_wait(&i_full[it & 1], (it >> 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
+    item = items[it & 1];
+    return !__any_sync(0xffffffffu, item.more == 0 || *abort_flag != 0);
+  };
+  auto release_item = [&](int it) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&i_empty[it & 1]);
+  };
 
   if (warp == 0) {
-    if (lane == 0) {
+    {
       int g = 0;  // streamed tiles loaded so far (ring position)
-      Walk walk = start();
-      Item item;
-      for (int it = 0; next(walk, item); ++it) {
+      BwdItem item;
+      for (int it = 0; take_item(it, item); ++it) {
+        release_item(it);
+        if (lane != 0) continue;
         const int rt = item.rt, b = item.b, h = item.h, t_begin = item.t_begin, n_t = item.n_t;
         mbar_wait(r_empty, (it & 1) ^ 1u, wctx, STATUS_TIMEOUT_PIPE_EMPTY);  // previous item's score MMAs done
         mbar_arrive_expect_tx(r_full, 2 * R_BYTES);
@@ -290,7 +280,7 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
           }
         }
       }
-      settle_copies(wctx);
+      if (lane == 0) settle_copies(wctx);
     }
   } else if (warp == 1) {
     // Score MMAs (whole warp, converged: the MMA / commit helpers elect the issuing lane); runs ahead as
@@ -298,11 +288,11 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     constexpr uint32_t idesc_xy = umma_idesc_bf16(128, 64, 0, 0);
     const uint32_t r1 = smem_u32(R1), r2 = smem_u32(R2);
     int g = 0;
-    Walk walk = start();
-    Item item;
-    for (int it = 0; next(walk, item); ++it) {
+    BwdItem item;
+    for (int it = 0; take_item(it, item); ++it) {
+      release_item(it);
       const int b = item.b, t_begin = item.t_begin, n_t = item.n_t;
-      const bool padded = p.mask.padded[b] != 0;
+      const bool padded = item.padded != 0;
       const int n = n_t * hpi;
       mbar_wait(r_full, it & 1, wctx, STATUS_TIMEOUT_PIPE_FULL);
       for (int t = 0; t < n; ++t, ++g) {
@@ -325,9 +315,9 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     // gradient MMAs
     constexpr uint32_t idesc_acc = umma_idesc_bf16(128, D, 0, 1);
     int g = 0;
-    Walk walk = start();
-    Item item;
-    for (int it = 0; next(walk, item); ++it) {
+    BwdItem item;
+    for (int it = 0; take_item(it, item); ++it) {
+      release_item(it);
       const int n = item.n_t * hpi;
       for (int t = 0; t < n; ++t, ++g) {
         const int st = g % TS, sb = g & 1;
@@ -348,7 +338,61 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
       }
       umma_commit_e(acc_full);
     }
-  } else if (warp >= MBWD_FIRST_CW) {
+  } else if (warp == 3) {
+    const int heads = MODE == 0 ? p.nh / p.group : p.nh;
+    const int BHP = p.B * heads * p.parts;
+    const int4* const plans = MODE == 0 ? p.mask.plan_k : p.mask.plan_q;
+    const int G = static_cast<int>(gridDim.x);
+    for (int it = 0;; ++it) {
+      const int w = it * G + ((it & 1) ? G - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
+      const bool more = w < n_items;       // an item past the end can only occur in a CTA's last round
+      int4 plan = make_int4(0, 0, 0, 0);
+      int b = 0, h = 0, part = 0;
+      BwdRows* rows = &item_rows[it & 1];
+      int lo[4], hi[4];
+      float lse[4] = {}, dvec[4] = {};
+      if (more) {
+        const int level = w / BHP;
+        int q = w - level * BHP;
+        part = q % p.parts;
+        q /= p.parts;
+        b = q / heads;
+        h = q - b * heads;
+        plan = plans[static_cast<size_t>(b) * n_rt + level];
+        if (Shape::ROWS) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = plan.x * 128 + 32 * i + lane;
+            lo[i] = lo_all[static_cast<size_t>(b) * p.S_pad + row];
+            hi[i] = hi_all[static_cast<size_t>(b) * p.S_pad + row];
+            if (MODE == 1) {
+              lse[i] = p.lse[(static_cast<size_t>(b) * p.nh + h) * p.S_pad + row];
+              dvec[i] = p.dvec[(static_cast<size_t>(b) * p.nh + h) * p.S_pad + row];
+            }
+          }
+        }
+      }
+      mbar_wait(&i_empty[it & 1], ((it >> 1) & 1) ^ 1u, wctx, STATUS_TIMEOUT_PIPE_EMPTY);
+      if (more && Shape::ROWS) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          rows->lo[32 * i + lane] = lo[i];
+          rows->hi[32 * i + lane] = hi[i];
+          if (MODE == 1) {
+            rows->lse[32 * i + lane] = lse[i];
+            rows->dvec[32 * i + lane] = dvec[i];
+          }
+        }
+      }
+      if (lane == 0) {
+        const int t_begin = plan.y >> 6;
+        items[it & 1] = BwdItem{more, b, h, plan.x, part, plan.w, t_begin, max(((plan.z + 63) >> 6) - t_begin, 1)};
+      }
+      __syncwarp();
+      mbar_arrive(&i_full[it & 1]);
+      if (!more || __any_sync(0xffffffffu, *abort_flag != 0)) break;
+    }
+  } else {
     const int cw = warp - MBWD_FIRST_CW;
     const int quarter = warp & 3;
     const int half = (cw >> 2) & 1;     // 32 of the 64 streamed columns
@@ -364,25 +408,37 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     uint8_t* stage = staging + cw * Shape::STAGE_BYTES;
     bool acc_pending = false;           // the previous item's acc_full phase has not been waited for
     int g0 = 0;
-    Walk walk = start();
-    Item item;
-    for (int it = 0; next(walk, item); ++it) {
+    BwdItem item;
+    for (int it = 0; take_item(it, item); ++it) {
       const int rt = item.rt, b = item.b, h = item.h, t_begin = item.t_begin, n_t = item.n_t;
       const int head0 = MODE == 0 ? h * p.group + item.part * hpi : h;   // query head of the item's first tiles
       const int n = n_t * hpi;
       const int row_g = rt * 128 + r;  // mode 0: key position, mode 1: query position
-      const int* lo_b = lo_all + static_cast<size_t>(b) * p.S_pad;
-      const int* hi_b = hi_all + static_cast<size_t>(b) * p.S_pad;
-      const int lo = lo_b[row_g], hi = hi_b[row_g];
-      const int row0 = rt * 128 + quarter * 32, row_z = min(row0 + 31, p.S - 1);
-      // what every row of this warp sees, and what any of them does (a warp past the end: nothing)
-      const int lo_min = lo_b[row0], hi_min = hi_b[row0];
-      const int lo_max = row0 < p.S ? lo_b[row_z] : lo_min, hi_max = row0 < p.S ? hi_b[row_z] : hi_min;
+      int lo, hi;
       float row_lse = 0.f, row_dvec = 0.f;
-      if (MODE == 1) {
-        row_lse = p.lse[(static_cast<size_t>(b) * p.nh + h) * p.S_pad + row_g];
-        row_dvec = p.dvec[(static_cast<size_t>(b) * p.nh + h) * p.S_pad + row_g];
+      if (Shape::ROWS) {
+        const BwdRows& rows = item_rows[it & 1];
+        lo = rows.lo[r];
+        hi = rows.hi[r];
+        if (MODE == 1) {
+          row_lse = rows.lse[r];
+          row_dvec = rows.dvec[r];
+        }
+      } else {
+        const size_t at = static_cast<size_t>(b) * p.S_pad + row_g;
+        lo = lo_all[at];
+        hi = hi_all[at];
+        if (MODE == 1) {
+          row_lse = p.lse[(static_cast<size_t>(b) * p.nh + h) * p.S_pad + row_g];
+          row_dvec = p.dvec[(static_cast<size_t>(b) * p.nh + h) * p.S_pad + row_g];
+        }
       }
+      release_item(it);
+      const int row0 = rt * 128 + quarter * 32;
+      // what every row of this warp sees, and what any of them does (a warp past the end: nothing)
+      const int z = max(min(31, p.S - 1 - row0), 0);
+      const int lo_min = __shfl_sync(0xffffffffu, lo, 0), hi_min = __shfl_sync(0xffffffffu, hi, 0);
+      const int lo_max = __shfl_sync(0xffffffffu, lo, z), hi_max = __shfl_sync(0xffffffffu, hi, z);
       for (int t = (g0 + group) & 1; t < n; t += 2) {
         const int g = g0 + t;
         const int st = g % TS;                      // streamed-tile stage (for the column statistics)
@@ -511,7 +567,7 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
         }
         if (MODE == 0 && p.parts > 1) {
           // fp32, one part of the sum: 16 columns at a time, the width of a staged row
-          float* to = p.partial + (((static_cast<size_t>(item.part) * 2 + is_dv) * p.B + b) * heads + h) * p.S_pad * D +
+          float* to = p.partial + (((static_cast<size_t>(item.part) * 2 + is_dv) * p.B + b) * (p.nh / p.group) + h) * p.S_pad * D +
                       static_cast<size_t>(row0) * D + c;
 #pragma unroll
           for (int c2 = 0; c2 < 2; ++c2) {
