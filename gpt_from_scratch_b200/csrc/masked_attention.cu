@@ -483,7 +483,9 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
           mma_kk<D / 16>(s_tmem + buf * 64, q_addr, 16384, smem_u32(Ks + st * KV_TILE), 8192, idesc_s, false);
           umma_commit_e(&s_full[2 * x + buf]);
           umma_commit_e(&k_empty[st]);
+          if (j + 1 == j1) umma_commit_e(&q_empty[x]);      // the tile's last: the next item's queries may come
         };
+        if (j1 <= j0) umma_commit_e(&q_empty[x]);
         auto values = [&](int j) {
           const int g = g0 + j - u0, st = g % KS, n = cx + j - j0, buf = n & 1;
           mbar_wait(&v_full[st], (g / KS) & 1, wctx, STATUS_TIMEOUT_PIPE_FULL);
@@ -503,7 +505,6 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
         scores(u0);
         if (u0 + 1 < u1) scores(u0 + 1);
         for (int j = u0; j < u1; ++j) {
-          if (j == max(u1 - 2, u0)) umma_commit_e(&q_empty[x]);  // all scores of the item have been issued
           values(j);
           if (j + 2 < u1) scores(j + 2);
         }

@@ -545,7 +545,6 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
       const int c0 = (MODE == 0) ? half * (D / 2) : (D == 128 ? group * 64 + half * 32 : half * 32);
       const bool is_dv = MODE == 0 && group == 1;
       const float out_scale = is_dv ? 1.f : (CAP ? 4.f : 1.f) * p.scale;
-      const bool seen = lo < hi;                       // padding: zeros, whatever its own rows held
       const long long o_ss = is_dv ? p.o2_ss : p.o1_ss;
       __nv_bfloat16* out = is_dv ? p.out2 + row0 * p.o2_ss + b * p.o2_bs + h * p.o2_hs
                                  : p.out1 + row0 * p.o1_ss + b * p.o1_bs + h * p.o1_hs;
@@ -565,6 +564,10 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
           __syncwarp();
           if (lane == 0) mbar_arrive(acc_empty);
         }
+        if (item.padded != 0 && lo >= hi) {    // padding: zeros, whatever its own rows held
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0u;
+        }
         if (MODE == 0 && p.parts > 1) {
           // fp32, one part of the sum: 16 columns at a time, the width of a staged row
           float* to = p.partial + (((static_cast<size_t>(item.part) * 2 + is_dv) * p.B + b) * (p.nh / p.group) + h) * p.S_pad * D +
@@ -573,13 +576,16 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
           for (int c2 = 0; c2 < 2; ++c2) {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              wv[e] = seen ? __float_as_uint(__uint_as_float(v[16 * c2 + e]) * out_scale) : 0u;
+              wv[e] = __float_as_uint(__uint_as_float(v[16 * c2 + e]) * out_scale);
             store_rows_32x32(stage, wv, lane, reinterpret_cast<__nv_bfloat16*>(to + 16 * c2), 2 * D, p.S - row0);
           }
         } else {
+          const uint64_t scale2 = pack_f32x2(out_scale, out_scale);
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            wv[e] = seen ? pack_bf16x2(__uint_as_float(v[2 * e]) * out_scale, __uint_as_float(v[2 * e + 1]) * out_scale) : 0u;
+          for (int e = 0; e < 16; ++e) {
+            const float2 o = unpack_f32x2(mul_f32x2(pack_u32x2(v[2 * e], v[2 * e + 1]), scale2));
+            wv[e] = pack_bf16x2(o.x, o.y);
+          }
           store_rows_32x32(stage, wv, lane, out + c, o_ss, p.S - row0);
         }
       }
