@@ -495,6 +495,31 @@ template <int N>
 __device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+// Cluster launch control: a running CTA takes over the work of one of the grid's that has not started. claim_cta asks (one
+// thread; 16 bytes arrive at `result`, 16-byte aligned, and are counted on `bar`); claimed_cta reads the answer: whether there was
+// one, and its blockIdx.x. After a refusal nobody asks again. Each CTA of a grid runs or is claimed, once.
+__device__ __forceinline__ void claim_cta(void* result, uint64_t* bar) {
+  mbar_arrive_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(result)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ bool claimed_cta(const void* result, int& block) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t.reg .b32 y, z, u;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, u}, r;\n\t}"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_u32(result))
+      : "memory");
+  block = static_cast<int>(x);
+  return ok != 0;
+}
 __device__ __forceinline__ bool elect_one() {
   uint32_t pred;
   asm volatile(

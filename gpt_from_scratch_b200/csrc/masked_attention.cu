@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(MASK_THREADS) attention_mask_kernel(const Mask
 }
 
 // ---------------------------------------------------------------------------
-// Forward. One persistent CTA per SM walks items of two tiles of 128 queries that share the loads of their keys: two heads of a
+// Forward. An item is a CTA of the grid; those that run (one per SM) claim further ones, the widest first. It is two tiles of 128 queries that share the loads of their keys: two heads of a
 // group at the same queries (groups of an even number), else neighbouring tiles of a head. A thread per query row.
 // ---------------------------------------------------------------------------
 struct MaskedFwdParams {
@@ -309,8 +309,9 @@ constexpr int MFWD_SW = 8;                          // four per tile, a row per 
 constexpr int MFWD_THREADS = 32 * (MFWD_FIRST_SW + MFWD_SW);
 // 384 threads x 168 at the launch = 128 x 72 + 256 x 216: a softmax thread holds the scores of two blocks of its row.
 constexpr int MFWD_REGS_IO = 72, MFWD_REGS_SOFTMAX = 216;
-// A work item, as warp 3 puts it into shared memory one ahead of the others: nobody else divides or waits for the plans.
+// A work item, as warp 3 puts it into shared memory when the one before has been taken: nobody else divides or waits for the plans.
 struct alignas(16) FwdItem {
+  uint4 claim;                 // what claim_cta answered
   int more;                    // 0: there are no further items
   int b, padded;
   int h[2], row[2];            // heads and first query rows of the two tiles
@@ -325,7 +326,7 @@ struct MFwdShape {
   static constexpr int Q_TILE = DB * 16384, KV_TILE = DB * 8192;    // 128 queries, 64 keys
   static constexpr int KS = D == 64 ? 8 : 4;        // stages of K and V
   static constexpr int STAGING = MFWD_SW * 2048;    // to transpose the output rows through
-  static constexpr int SMEM = 2 * Q_TILE + 2 * KS * KV_TILE + STAGING + 2 * sizeof(FwdItem) + 512;
+  static constexpr int SMEM = 2 * Q_TILE + 2 * KS * KV_TILE + STAGING + sizeof(FwdItem) + 512;
 };
 // Scores: as they are, capped with a bound that the running maximum may be left out for, capped.
 enum Scores { PLAIN = 0, BOUNDED = 1, CAPPED = 2 };
@@ -336,7 +337,7 @@ constexpr float BOUNDED_CAP2 = 80.f;
 template <int D, int SCORES, bool DIST>
 __global__ void __launch_bounds__(MFWD_THREADS, 1)
 masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                  const __grid_constant__ CUtensorMap tv, const MaskedFwdParams p, int n_levels, int n_items) {
+                  const __grid_constant__ CUtensorMap tv, const MaskedFwdParams p, int n_levels) {
   using Shape = MFwdShape<D>;
   constexpr int DB = Shape::DB, Q_TILE = Shape::Q_TILE, KV_TILE = Shape::KV_TILE, KS = Shape::KS;
   constexpr uint32_t O_COL = 256;            // scores at [tile][buffer][64] before that; P takes the columns of its scores
@@ -345,8 +346,8 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
   uint8_t* Ks = Qs + 2 * Q_TILE;             // [KS]
   uint8_t* Vs = Ks + KS * KV_TILE;           // [KS]
   uint8_t* staging = Vs + KS * KV_TILE;
-  FwdItem* items = reinterpret_cast<FwdItem*>(staging + Shape::STAGING);   // [2]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(items + 2);
+  FwdItem& item = *reinterpret_cast<FwdItem*>(staging + Shape::STAGING);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(&item + 1);
   uint64_t* q_full = bars;                   // [tile]
   uint64_t* q_empty = bars + 2;
   uint64_t* k_full = bars + 4;               // [KS]
@@ -357,9 +358,10 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
   uint64_t* p_full = s_full + 4;
   uint64_t* o_full = p_full + 4;             // P V of the buffer is done
   uint64_t* o_empty = o_full + 4;            // [tile]
-  uint64_t* i_full = o_empty + 2;            // [2]
-  uint64_t* i_empty = i_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(i_empty + 2);
+  uint64_t* i_full = o_empty + 2;
+  uint64_t* i_empty = i_full + 1;
+  uint64_t* i_claim = i_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(i_full + 3);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -381,11 +383,10 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       mbar_init(&p_full[i], MFWD_SW / 2);
       mbar_init(&o_full[i], 1);
     }
-    for (int x = 0; x < 2; ++x) {
-      mbar_init(&o_empty[x], MFWD_SW / 2);
-      mbar_init(&i_full[x], 32);
-      mbar_init(&i_empty[x], 3 + MFWD_SW);
-    }
+    for (int x = 0; x < 2; ++x) mbar_init(&o_empty[x], MFWD_SW / 2);
+    mbar_init(i_full, 32);
+    mbar_init(i_empty, 3 + MFWD_SW);
+    mbar_init(i_claim, 1);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tq);
@@ -404,15 +405,15 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
   const uint32_t tmem_base = *tmem_slot;
   WaitCtx wctx{abort_flag, p.status, GFS_WAIT_LIMIT_NS};
 
-  // Items: the widest first, dealt to the CTAs in a snake; all barrier parities run on counters that continue across items.
-  // What a warp wants of the it-th item it copies out of its slot, then it releases the slot.
+  // All barrier parities run on counters that continue across items. What a warp wants of the it-th item it copies out of the
+  // slot, then it releases it.
   auto take_item = [&](int it) {        // false, for the whole warp: there are no more, or a wait has given up
-    mbar_wait(&i_full[it & 1], (it >> 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
-    return !__any_sync(0xffffffffu, items[it & 1].more == 0 || *abort_flag != 0);
+    mbar_wait(i_full, it & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
+    return !__any_sync(0xffffffffu, item.more == 0 || *abort_flag != 0);
   };
-  auto release_item = [&](int it) {
+  auto release_item = [&]() {
     __syncwarp();
-    if (lane == 0) mbar_arrive(&i_empty[it & 1]);
+    if (lane == 0) mbar_arrive(i_empty);
   };
   struct Blocks {
     int u0, u1;      // all blocks of the item
@@ -426,10 +427,8 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
     if (warp == 0) {
       int g = 0;      // key blocks loaded so far (ring position)
       for (int it = 0; take_item(it); ++it) {
-        const FwdItem& item = items[it & 1];
         const int bb = item.b, kvh = item.h[0] / p.group;
         const Blocks u = blocks_of(item);
-        release_item(it);
         if (lane == 0) {
           for (int j = u.u0; j < u.u1; ++j, ++g) {
             const int st = g % KS;
@@ -446,6 +445,9 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
               tma_load_4d(Vs + st * KV_TILE + db * 8192, &tv, &v_full[st], db * 64, j * 64, kvh, bb);
           }
         }
+        // Only now may the next item be claimed: one that is claimed early waits here while other SMs have run out of work (us:
+        // 64 heads of 4096 tokens under a window 224 -> 234 with the release at the start).
+        release_item();
       }
       if (lane == 0) settle_copies(wctx);
     } else if (warp <= 2) {
@@ -463,12 +465,11 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       int cx = 0;               // this tile's blocks in earlier items (barrier phases)
       int had = 0;              // items in which it had blocks (phase of o_empty)
       for (int it = 0; take_item(it); ++it) {
-        const FwdItem& item = items[it & 1];
         const int u0 = blocks_of(item).u0, u1 = blocks_of(item).u1;
         const int j0 = item.j0[x], j1 = item.j1[x];
         const bool padded = item.padded != 0;
         const int *first = p.mask.first + static_cast<size_t>(item.b) * p.S_pad, *last = p.mask.last + static_cast<size_t>(item.b) * p.S_pad;
-        release_item(it);
+        release_item();
         mbar_wait(&q_full[x], it & 1, wctx, STATUS_TIMEOUT_PIPE_FULL);
         auto scores = [&](int j) {
           const int g = g0 + j - u0, st = g % KS, n = cx + j - j0, buf = n & 1;
@@ -515,12 +516,16 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
     } else {
       const int heads = p.head_pairs ? p.nh / 2 : p.nh;
       const int BH = p.B * heads;
-      const int G = static_cast<int>(gridDim.x);
       for (int it = 0;; ++it) {
-        const int w = it * G + ((it & 1) ? G - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
-        const bool more = w < n_items;       // an item past the end can only occur in a CTA's last round
-        mbar_wait(&i_empty[it & 1], ((it >> 1) & 1) ^ 1u, wctx, STATUS_TIMEOUT_PIPE_EMPTY);
-        FwdItem& item = items[it & 1];
+        mbar_wait(i_empty, (it & 1) ^ 1u, wctx, STATUS_TIMEOUT_PIPE_EMPTY);
+        int w = blockIdx.x;
+        bool more = true;
+        if (it > 0) {
+          if (lane == 0) claim_cta(&item.claim, i_claim);
+          more = mbar_wait(i_claim, (it - 1) & 1, wctx, STATUS_TIMEOUT_PIPE_FULL) && claimed_cta(&item.claim, w);
+          more = __all_sync(0xffffffffu, more);
+          fence_proxy_async_smem();      // the next answer comes after everybody has read this one
+        }
         if (more) {
           const int bh = w % BH, b = bh / heads, h = bh % heads;
           const size_t at = static_cast<size_t>(b) * n_levels + w / BH;
@@ -576,7 +581,7 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
         }
         if (lane == 0) item.more = more;
         __syncwarp();
-        mbar_arrive(&i_full[it & 1]);
+        mbar_arrive(i_full);
         if (!more || __any_sync(0xffffffffu, *abort_flag != 0)) break;
         if (lane == 0) {
           for (int x = 0; x < 2; ++x) {        // (rows past S: zeros)
@@ -651,10 +656,9 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
     };
     int cdone = 0;  // blocks of this tile processed in earlier items
     for (int it = 0; take_item(it); ++it) {
-      const FwdItem& item = items[it & 1];
       const Rows q{item.lo[x][r], item.hi[x][r], item.lo_max[x], item.hi_min[x], item.slope2[x]};
       const int j0 = item.j0[x], j1 = item.j1[x], row = item.row[x] + r, b = item.b, h = item.h[x];
-      release_item(it);
+      release_item();
       float m = MAXED ? -INFINITY : 0.f;
       uint64_t l2 = 0, t2 = 0;                  // sums of the probabilities, as they are and as rounded to bf16
       // 32 exponents -> probabilities, packed, and their sums
@@ -795,9 +799,9 @@ int launch_fwd(const CUtensorMap* tq, const CUtensorMap* tk, const CUtensorMap* 
   if (!limit.raise(masked_fwd_kernel<D, SCORES, DIST>, smem)) return -10;
   const int tiles = p.S_pad / 128;
   const int n_levels = p.head_pairs ? tiles : (tiles + 1) / 2;
-  const int n_items = n_levels * p.B * (p.head_pairs ? p.nh / 2 : p.nh);
-  gfs_host::launch_pdl(masked_fwd_kernel<D, SCORES, DIST>, dim3(std::min(n_items, gfs_host::sm_count())), dim3(MFWD_THREADS),
-                       smem, stream, *tq, *tk, *tv, p, n_levels, n_items);
+  const unsigned n_items = static_cast<unsigned>(n_levels) * p.B * (p.head_pairs ? p.nh / 2 : p.nh);
+  gfs_host::launch_pdl(masked_fwd_kernel<D, SCORES, DIST>, dim3(n_items), dim3(MFWD_THREADS), smem, stream, *tq, *tk,
+                       *tv, p, n_levels);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 template <int D, bool DIST>

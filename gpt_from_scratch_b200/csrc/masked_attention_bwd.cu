@@ -110,9 +110,10 @@ constexpr int MBWD_CW = 16;                         // compute warps
 constexpr int MBWD_FIRST_CW = 4;                    // warps 0-2: TMA, score MMAs, gradient MMAs; 3: items
 constexpr int MBWD_THREADS = 32 * (MBWD_FIRST_CW + MBWD_CW);
 
-// A work item, as warp 3 puts it into shared memory one ahead of the others: nobody else divides or waits for the plans. At
+// A work item, as warp 3 puts it into shared memory when the one before has been taken: nobody else divides or waits for the plans. At
 // head_dim 64 there is room for what the resident rows see and (mode 1) their statistics too.
 struct alignas(16) BwdItem {
+  uint4 claim;                 // what claim_cta answered
   int more;                    // 0: there are no further items
   int b, h, rt, part, padded;
   int t_begin, n_t;            // streamed tiles per head (at least one, which may be masked whole)
@@ -130,7 +131,7 @@ struct MBwdShape {
   static constexpr int STAGE_BYTES = 2048;          // per compute warp, to transpose its output rows through
   static constexpr int STAGING = MBWD_CW * STAGE_BYTES;
   static constexpr bool ROWS = D == 64;             // BwdRows beside the items
-  static constexpr int ITEMS = 2 * static_cast<int>(sizeof(BwdItem) + (ROWS ? sizeof(BwdRows) : 0));
+  static constexpr int ITEMS = static_cast<int>(sizeof(BwdItem) + (ROWS ? sizeof(BwdRows) : 0));
   static constexpr int SMEM = 2 * (D / 64) * 16384 + 2 * TS * (D / 64) * 8192 + STAGING + (MODE == 0 ? TS * 512 : 0) + ITEMS + 256;
 };
 
@@ -142,7 +143,7 @@ template <int D, int MODE, bool CAP, bool DIST>
 __global__ void __launch_bounds__(MBWD_THREADS, 1)
 masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant__ CUtensorMap tr2,
                   const __grid_constant__ CUtensorMap tt1, const __grid_constant__ CUtensorMap tt2,
-                  const MaskedBwdParams p, int n_rt, int n_items) {
+                  const MaskedBwdParams p, int n_rt) {
   using Shape = MBwdShape<D, MODE>;
   constexpr int DB = D / 64;
   constexpr int TS = Shape::TS;
@@ -161,9 +162,9 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
   uint8_t* T2 = T1 + TS * T_BYTES;
   uint8_t* staging = T2 + TS * T_BYTES;
   float* stats = reinterpret_cast<float*>(staging + Shape::STAGING);  // mode 0: [TS stages][lse 64 | dvec 64]
-  BwdItem* items = reinterpret_cast<BwdItem*>(reinterpret_cast<uint8_t*>(stats) + (MODE == 0 ? TS * 512 : 0));   // [2]
-  BwdRows* item_rows = reinterpret_cast<BwdRows*>(items + 2);                                                 // [2]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(items) + Shape::ITEMS);
+  BwdItem* slot = reinterpret_cast<BwdItem*>(reinterpret_cast<uint8_t*>(stats) + (MODE == 0 ? TS * 512 : 0));
+  BwdRows* rows = reinterpret_cast<BwdRows*>(slot + 1);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(slot) + Shape::ITEMS);
   uint64_t* r_full = bars;
   uint64_t* t_full = bars + 1;             // [TS]
   uint64_t* t_empty = t_full + TS;         // [TS]
@@ -174,9 +175,10 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
   uint64_t* acc_full = m_empty + 2;
   uint64_t* acc_empty = acc_full + 1;
   uint64_t* r_empty = acc_full + 2;
-  uint64_t* i_full = acc_full + 3;         // [2]
-  uint64_t* i_empty = i_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(i_empty + 2);
+  uint64_t* i_full = acc_full + 3;
+  uint64_t* i_empty = i_full + 1;
+  uint64_t* i_claim = i_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(i_full + 3);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -188,8 +190,8 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
   // the rows that a resident row sees: queries of a key, keys of a query
   const int* const lo_all = MODE == 0 ? p.mask.qfirst : p.mask.first;
   const int* const hi_all = MODE == 0 ? p.mask.qlast : p.mask.last;
-  // Persistent: a CTA walks work items (resident tile, batch * head * part), the heaviest first, dealt in a snake over the
-  // CTAs; barrier phases run on counters that continue across items, so the next item's loads and first score MMAs overlap
+  // An item (resident tile, batch * head * part) is a CTA of the grid, the heaviest first; those that run (one per SM) claim
+  // further ones. Barrier phases run on counters that continue across items, so the next item's loads and first score MMAs overlap
   // this one's epilogue.
   const int hpi = MODE == 0 ? p.group / p.parts : 1;    // heads per item
 
@@ -208,10 +210,9 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, EPI_WARPS);
     mbar_init(r_empty, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&i_full[i], 32);
-      mbar_init(&i_empty[i], 3 + MBWD_CW);
-    }
+    mbar_init(i_full, 32);
+    mbar_init(i_empty, 3 + MBWD_CW);
+    mbar_init(i_claim, 1);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tr1);
@@ -233,24 +234,23 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
   pdl_trigger();
   const uint32_t tmem_base = *tmem_slot;
   WaitCtx wctx{abort_flag, p.status, GFS_WAIT_LIMIT_NS};
-  // The it-th item is copied out of its slot and the slot released; false, for the whole warp: there are no more, or a wait has
+  // The it-th item is copied out of the slot and the slot released; false, for the whole warp: there are no more, or a wait has
   // given up.
   auto take_item = [&](int it, BwdItem& item) {
-    mbar_wait(&i_full[it & 1], (it >> 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
-    item = items[it & 1];
+    mbar_wait(i_full, it & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
+    item = *slot;
     return !__any_sync(0xffffffffu, item.more == 0 || *abort_flag != 0);
   };
-  auto release_item = [&](int it) {
+  auto release_item = [&]() {
     __syncwarp();
-    if (lane == 0) mbar_arrive(&i_empty[it & 1]);
+    if (lane == 0) mbar_arrive(i_empty);
   };
 
   if (warp == 0) {
     {
       int g = 0;  // streamed tiles loaded so far (ring position)
       BwdItem item;
-      for (int it = 0; take_item(it, item); ++it) {
-        release_item(it);
+      for (int it = 0; take_item(it, item); ++it, release_item()) {     // released, so the next one claimed, after the loads
         if (lane != 0) continue;
         const int rt = item.rt, b = item.b, h = item.h, t_begin = item.t_begin, n_t = item.n_t;
         mbar_wait(r_empty, (it & 1) ^ 1u, wctx, STATUS_TIMEOUT_PIPE_EMPTY);  // previous item's score MMAs done
@@ -290,7 +290,7 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     int g = 0;
     BwdItem item;
     for (int it = 0; take_item(it, item); ++it) {
-      release_item(it);
+      release_item();
       const int b = item.b, t_begin = item.t_begin, n_t = item.n_t;
       const bool padded = item.padded != 0;
       const int n = n_t * hpi;
@@ -317,7 +317,7 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     int g = 0;
     BwdItem item;
     for (int it = 0; take_item(it, item); ++it) {
-      release_item(it);
+      release_item();
       const int n = item.n_t * hpi;
       for (int t = 0; t < n; ++t, ++g) {
         const int st = g % TS, sb = g & 1;
@@ -342,13 +342,18 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     const int heads = MODE == 0 ? p.nh / p.group : p.nh;
     const int BHP = p.B * heads * p.parts;
     const int4* const plans = MODE == 0 ? p.mask.plan_k : p.mask.plan_q;
-    const int G = static_cast<int>(gridDim.x);
     for (int it = 0;; ++it) {
-      const int w = it * G + ((it & 1) ? G - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
-      const bool more = w < n_items;       // an item past the end can only occur in a CTA's last round
+      mbar_wait(i_empty, (it & 1) ^ 1u, wctx, STATUS_TIMEOUT_PIPE_EMPTY);
+      int w = blockIdx.x;
+      bool more = true;
+      if (it > 0) {
+        if (lane == 0) claim_cta(&slot->claim, i_claim);
+        more = mbar_wait(i_claim, (it - 1) & 1, wctx, STATUS_TIMEOUT_PIPE_FULL) && claimed_cta(&slot->claim, w);
+        more = __all_sync(0xffffffffu, more);
+        fence_proxy_async_smem();      // the next answer comes after everybody has read this one
+      }
       int4 plan = make_int4(0, 0, 0, 0);
       int b = 0, h = 0, part = 0;
-      BwdRows* rows = &item_rows[it & 1];
       int lo[4], hi[4];
       float lse[4] = {}, dvec[4] = {};
       if (more) {
@@ -372,7 +377,6 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
           }
         }
       }
-      mbar_wait(&i_empty[it & 1], ((it >> 1) & 1) ^ 1u, wctx, STATUS_TIMEOUT_PIPE_EMPTY);
       if (more && Shape::ROWS) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -386,12 +390,20 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
       }
       if (lane == 0) {
         const int t_begin = plan.y >> 6;
-        items[it & 1] = BwdItem{more, b, h, plan.x, part, plan.w, t_begin, max(((plan.z + 63) >> 6) - t_begin, 1)};
+        slot->more = more;
+        slot->b = b;
+        slot->h = h;
+        slot->rt = plan.x;
+        slot->part = part;
+        slot->padded = plan.w;
+        slot->t_begin = t_begin;
+        slot->n_t = max(((plan.z + 63) >> 6) - t_begin, 1);
       }
       __syncwarp();
-      mbar_arrive(&i_full[it & 1]);
+      mbar_arrive(i_full);
       if (!more || __any_sync(0xffffffffu, *abort_flag != 0)) break;
     }
+    if (lane == 0) settle_copies(wctx);
   } else {
     const int cw = warp - MBWD_FIRST_CW;
     const int quarter = warp & 3;
@@ -417,12 +429,11 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
       int lo, hi;
       float row_lse = 0.f, row_dvec = 0.f;
       if (Shape::ROWS) {
-        const BwdRows& rows = item_rows[it & 1];
-        lo = rows.lo[r];
-        hi = rows.hi[r];
+        lo = rows->lo[r];
+        hi = rows->hi[r];
         if (MODE == 1) {
-          row_lse = rows.lse[r];
-          row_dvec = rows.dvec[r];
+          row_lse = rows->lse[r];
+          row_dvec = rows->dvec[r];
         }
       } else {
         const size_t at = static_cast<size_t>(b) * p.S_pad + row_g;
@@ -433,7 +444,7 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
           row_dvec = p.dvec[(static_cast<size_t>(b) * p.nh + h) * p.S_pad + row_g];
         }
       }
-      release_item(it);
+      release_item();
       const int row0 = rt * 128 + quarter * 32;
       // what every row of this warp sees, and what any of them does (a warp past the end: nothing)
       const int z = max(min(31, p.S - 1 - row0), 0);
@@ -648,11 +659,11 @@ int launch_bwd(const BwdMaps& m, const MaskedBwdParams& p0, const MaskedBwdParam
   constexpr int smem0 = MBwdShape<D, 0>::SMEM, smem1 = MBwdShape<D, 1>::SMEM;
   if (!limit0.raise(masked_bwd_kernel<D, 0, CAP, DIST>, smem0) || !limit1.raise(masked_bwd_kernel<D, 1, CAP, DIST>, smem1))
     return -10;
-  gfs_host::launch_pdl(masked_bwd_kernel<D, 0, CAP, DIST>, dim3(std::min(items0, gfs_host::sm_count())),
-                       dim3(MBWD_THREADS), smem0, stream, *m.k128, *m.v128, *m.q64, *m.do64, p0, n_rt, items0);
+  gfs_host::launch_pdl(masked_bwd_kernel<D, 0, CAP, DIST>, dim3(items0), dim3(MBWD_THREADS), smem0, stream, *m.k128,
+                       *m.v128, *m.q64, *m.do64, p0, n_rt);
   if (cudaGetLastError() != cudaSuccess) return -12;
-  gfs_host::launch_pdl(masked_bwd_kernel<D, 1, CAP, DIST>, dim3(std::min(items1, gfs_host::sm_count())),
-                       dim3(MBWD_THREADS), smem1, stream, *m.q128, *m.do128, *m.k64, *m.v64, p1, n_rt, items1);
+  gfs_host::launch_pdl(masked_bwd_kernel<D, 1, CAP, DIST>, dim3(items1), dim3(MBWD_THREADS), smem1, stream, *m.q128,
+                       *m.do128, *m.k64, *m.v64, p1, n_rt);
   return cudaGetLastError() == cudaSuccess ? 0 : -13;
 }
 template <int D>
