@@ -45,9 +45,8 @@ __global__ void __launch_bounds__(256) masked_dvec_kernel(const DvecArgs a) {
   const int sub = threadIdx.x & 7, b = blockIdx.y;
   const unsigned total = static_cast<unsigned>(a.S_pad) * a.nh;
   const unsigned row0 = blockIdx.x * (32u * DVEC_ROWS) + (threadIdx.x >> 3);
-  const bool padded = a.padded[b] != 0;
   uint4 x[DVEC_ROWS][V], y[DVEC_ROWS][V];
-  unsigned at[DVEC_ROWS];
+  unsigned at[DVEC_ROWS], token[DVEC_ROWS];
 #pragma unroll
   for (int i = 0; i < DVEC_ROWS; ++i) {
     const unsigned row = row0 + 32u * i;
@@ -55,10 +54,10 @@ __global__ void __launch_bounds__(256) masked_dvec_kernel(const DvecArgs a) {
     const unsigned rest = row - outer * a.inner;
     const unsigned s = a.s_fastest ? rest : outer, h = a.s_fastest ? outer : rest;
     at[i] = h * a.S_pad + s;
+    token[i] = min(s, static_cast<unsigned>(a.S_pad) - 1u);
 #pragma unroll
     for (int v = 0; v < V; ++v) x[i][v] = y[i][v] = make_uint4(0, 0, 0, 0);
-    const size_t m = static_cast<size_t>(b) * a.S_pad + s;
-    if (row < total && s < static_cast<unsigned>(a.S) && (!padded || a.first[m] < a.last[m])) {
+    if (row < total && s < static_cast<unsigned>(a.S)) {
       const __nv_bfloat16* px = a.dO + s * a.do_ss + b * a.do_bs + h * a.do_hs + sub * 8;
       const __nv_bfloat16* py = a.O + s * a.o_ss + b * a.o_bs + h * a.o_hs + sub * 8;
 #pragma unroll
@@ -68,6 +67,7 @@ __global__ void __launch_bounds__(256) masked_dvec_kernel(const DvecArgs a) {
       }
     }
   }
+  const bool padded = a.padded[b] != 0;       // (after the loads: they do not wait for it)
 #pragma unroll
   for (int i = 0; i < DVEC_ROWS; ++i) {
     float acc = 0.f;
@@ -83,6 +83,8 @@ __global__ void __launch_bounds__(256) masked_dvec_kernel(const DvecArgs a) {
     }
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    const size_t m = static_cast<size_t>(b) * a.S_pad + token[i];
+    if (padded && a.first[m] >= a.last[m]) acc = 0.f;
     if (row0 + 32u * i < total && sub == 0) a.dvec[static_cast<size_t>(b) * a.nh * a.S_pad + at[i]] = acc;
   }
 }
