@@ -808,8 +808,10 @@ template <int D, bool DIST>
 int launch_fwd_scores(const CUtensorMap* tq, const CUtensorMap* tk, const CUtensorMap* tv, const MaskedFwdParams& p,
                       cudaStream_t stream) {
   if (p.score.cap2 <= 0.f) return launch_fwd<D, PLAIN, DIST>(tq, tk, tv, p, stream);
-  return p.score.cap2 <= BOUNDED_CAP2 ? launch_fwd<D, BOUNDED, DIST>(tq, tk, tv, p, stream)
-                                      : launch_fwd<D, CAPPED, DIST>(tq, tk, tv, p, stream);
+  if constexpr (!DIST) {       // a bias has no bound: a slope may be negative
+    if (p.score.cap2 <= BOUNDED_CAP2) return launch_fwd<D, BOUNDED, false>(tq, tk, tv, p, stream);
+  }
+  return launch_fwd<D, CAPPED, DIST>(tq, tk, tv, p, stream);
 }
 
 }  // namespace

@@ -209,7 +209,7 @@ class _MaskedAttention(torch.autograd.Function):
         softcap, scale = ctx.args
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         if q.numel() == 0:
-            return dq, dk, dv, None, None, None, None
+            return dq, dk.zero_(), dv.zero_(), None, None, None, None
         B, nh, S, D = shape = q.shape
         kv = k.shape
         dout = _readable(dout)
@@ -235,8 +235,9 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
     Heads of q share those of k and v in groups of ``heads / kv_heads``. Scores are ``scale * q k`` (default ``1 / sqrt(D)``), with
     ``softcap`` c > 0 ``c tanh(scale * q k / c)``, with ``alibi_slopes`` (fp32 ``[heads]``, constants for autograd) minus
     ``slope * |i - j|``. A query that sees nothing gets zeros, and what padding holds does not matter; a value that is not
-    finite elsewhere may spread to queries of its 128-token tile that do not see it. On CUDA: bfloat16 and D 64 or 128, any
-    strides (copied first where a dimension is broadcast or 16-byte accesses do not reach), deterministic; other devices: torch operations.
+    finite elsewhere may spread to queries of its 128-token tile that do not see it. The result is laid out like q. On CUDA:
+    bfloat16, D 64 or 128 and softcap up to 1000, any strides (copied first where a dimension is broadcast or 16-byte accesses
+    do not reach), deterministic; other devices: torch operations.
     """
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError(f"masked_attention: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not fit")
@@ -262,6 +263,11 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
         if q.dtype != torch.bfloat16 or D not in (64, 128):
             raise ValueError(f"masked_attention: no native kernel for {q.dtype} and head_dim {D} (bfloat16 and 64 or 128 have "
                              "one); use masked_attention_reference for others")
+        if softcap and not 1e-6 <= softcap <= 1e3:
+            raise ValueError(f"masked_attention: softcap {softcap} is outside of 1e-6 to 1e3 (the error of a capped score is "
+                             "2^-22 of the cap)")
+        if B > 65535 or _pad128(S) * nh >= 2 ** 30 or _pad128(S) // 128 * B * nh >= 2 ** 31:
+            raise ValueError(f"masked_attention: {B} sequences of {S} tokens with {nh} heads are too many for one call")
         slopes = None if alibi_slopes is None else alibi_slopes.contiguous()
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
             return _MaskedAttention.apply(q, k, v, mask.buffer, slopes, float(softcap), float(scale))

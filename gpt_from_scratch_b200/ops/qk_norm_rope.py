@@ -99,6 +99,8 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: tor
     S, B, W = qkv.shape
     D = W // heads
     check_tables("qk_norm_rope", qkv, cos, sin, positions, S, B, D)
+    if not eps >= 0.0:
+        raise ValueError(f"qk_norm_rope: eps {eps} is negative")
     if (q_weight is None) != (k_weight is None):
         raise ValueError("qk_norm_rope: q and k are normalised both or not at all")
     for w in (q_weight, k_weight):

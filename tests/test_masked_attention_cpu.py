@@ -154,6 +154,6 @@ def test_rotary_refusals_and_reference():
     ops.qk_norm_rope(qkv, w, w, cos, sin, 3, 1)
     for args in ((qkv[0], w, w, cos, sin, 3, 1), (qkv, w, None, cos, sin, 3, 1), (qkv, w[:4], w, cos, sin, 3, 1),
                  (qkv, w.double(), w.double(), cos, sin, 3, 1), (qkv, w, w, cos, sin, 4, 1), (qkv, w, w, cos, sin, 0, 0),
-                 (qkv, w, w, cos, sin, -1, 3)):
+                 (qkv, w, w, cos, sin, -1, 3), (qkv, w, w, cos, sin, 3, 1, -1e-5), (qkv, w, w, cos, sin, 3, 1, float("nan"))):
         with pytest.raises(ValueError):
             ops.qk_norm_rope(*args)

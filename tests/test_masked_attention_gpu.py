@@ -237,6 +237,37 @@ def test_growing_and_large_scores(cuda_device, D):
     check(run(q, k, v, do, mask, scale=0.05), want, tols, "scale")
 
 
+@pytest.mark.parametrize("cap", [0.0, 10.0, 50.0, 900.0])
+def test_bias_that_grows_with_the_distance(cuda_device, cap):
+    """Negative slopes: far keys win by hundreds, so a capped score plus its bias has no bound."""
+    B, nh, S, D = 1, 3, 500, 64
+    q, k, v, do = tensors(B, nh, nh, S, D, 13, packed=False)
+    slopes = torch.tensor([-0.5, -2.0, 0.25], device=cuda_device)
+    mask = ops.attention_mask(B, S, device=cuda_device)
+    want, tols = bounds_and_values(q, k, v, do, mask.visible(), cap, slopes, 1 / 8)
+    check(run(q, k, v, do, mask, softcap=cap, alibi_slopes=slopes), want, tols, f"cap {cap}")
+
+
+def test_second_derivatives_are_refused(cuda_device):
+    q, k, v, do = tensors(1, 2, 2, 40, 64, 1, packed=False)
+    q = q.detach().requires_grad_()
+    out = ops.masked_attention(q, k, v, ops.attention_mask(1, 40, device=cuda_device))
+    dq, = torch.autograd.grad(out, q, do, create_graph=True)        # the first is computed as ever
+    assert torch.equal(dq, run(q, k, v, do, ops.attention_mask(1, 40, device=cuda_device))[1])
+    with pytest.raises(RuntimeError):
+        dq.float().sum().backward()
+
+
+def test_no_heads_and_gradients_of_some_inputs(cuda_device):
+    mask = ops.attention_mask(2, 70, device=cuda_device)
+    q, k, v, do = tensors(2, 4, 2, 70, 64, 1, packed=False)
+    k = k.detach().requires_grad_()
+    dk, = torch.autograd.grad(ops.masked_attention(q, k, v, mask), k, do)
+    assert torch.equal(dk, run(q, k, v, do, mask)[2])
+    dk, = torch.autograd.grad(ops.masked_attention(q[:, :0], k, v, mask), k, do[:, :0])
+    assert (dk == 0).all()
+
+
 def test_equals_causal_attention_of_the_framework(cuda_device):
     q, k, v, do = tensors(2, 3, 3, 512, 64, 3, packed=False)
     mask = ops.attention_mask(2, 512, device=cuda_device)
@@ -332,6 +363,12 @@ def test_empty_and_refused(cuda_device):
     t = torch.randn(1, 2, 8, 64, device=cuda_device).bfloat16()
     with pytest.raises(ValueError):
         ops.masked_attention(t, t, t, ops.attention_mask(1, 8))      # a mask on the CPU
+    for cap in (1e-9, 1e9):
+        with pytest.raises(ValueError):
+            ops.masked_attention(t, t, t, mask, softcap=cap)
+    many = t[:, :, :1].expand(70000, 2, 1, 64)
+    with pytest.raises(ValueError):
+        ops.masked_attention(many, many, many, ops.attention_mask(70000, 1, device=cuda_device))
     with pytest.raises(ValueError):
         ops.attention_mask(1, 8, document_ids=torch.zeros(1, 8, dtype=torch.int32), device=cuda_device)
 
