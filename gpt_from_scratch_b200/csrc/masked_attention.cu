@@ -17,8 +17,9 @@ using gfs_host::strides_ok;
 namespace {
 
 // ---------------------------------------------------------------------------
-// The mask. One CTA per sequence, a thread per token and step: running maxima from the left (where a document starts, the last token
-// that is not prefix) and running minima from the right (where it ends, the end of the prefix's run).
+// The mask. One CTA per sequence: running maxima from the left (where a document starts, the last token that is not prefix)
+// and running minima from the right (where it ends, the end of the prefix's run). Bound by latency, of the scans and of the few
+// loads and stores of one CTA: us, 6 for 16 x 1024 tokens, 11 for 2 x 4096 under a window, 16 for 8192 with documents and prefixes.
 // ---------------------------------------------------------------------------
 constexpr int MASK_THREADS = 1024;
 
@@ -84,7 +85,7 @@ __device__ __forceinline__ void sort_tiles(const int* lo, const int* hi, int S, 
 }
 
 // N: tokens per thread and step. A scan costs the same for 1,024 tokens as for 8,192 (1 -> 8 a thread, us: one sequence of 8192
-// with a prefix 30 -> 12; up to 2,048 tokens one a thread is as fast, and loads and stores are contiguous).
+// with a prefix 30 -> 16; up to 2,048 tokens one a thread has two steps at most, and needs no vectors).
 template <int N>
 __global__ void __launch_bounds__(MASK_THREADS) attention_mask_kernel(const MaskArgs a) {
   pdl_wait();
@@ -290,8 +291,23 @@ __global__ void __launch_bounds__(MASK_THREADS) attention_mask_kernel(const Mask
 }
 
 // ---------------------------------------------------------------------------
-// Forward. An item is a CTA of the grid; those that run (one per SM) claim further ones, the widest first. It is two tiles of 128 queries that share the loads of their keys: two heads of a
-// group at the same queries (groups of an even number), else neighbouring tiles of a head. A thread per query row.
+// Forward. An item is a CTA of the grid; those that run (one per SM) claim further ones, the widest first. It is two tiles
+// of 128 queries that share the loads of their keys: two heads of a group at the same queries (groups of an even number), else
+// neighbouring tiles of a head. Blocks of 64 keys, a thread per query row; scores double buffered in tensor memory, P over the
+// scores that it was made from, O beside them (2 x 2 x 64 + 2 x D columns).
+//
+// Bound by the softmax warps, two per scheduler: their exponentials keep the special function unit (16 a clock and SM) busy for
+// 45 % of the time, with a cap (2.25 operations a score) for 75 %; the rest is the length of their chains. us, and
+// products at a share of the measured tensor rate: 16 heads (4 of k) of 8192 tokens, head_dim 128, documents with prefixes 91
+// (0.41); 64 heads (16 of k) of 4096 under a window of 1024, capped 208 (0.35); 16 x 12 heads of 1024 tokens of head_dim 64 in
+// documents of 200 tokens, where an item is five blocks and every fourth score is needed, 48 (100 MB: 15 at copy speed).
+//
+// What led here, us for the three: a CTA per tile, two per SM, blocks of 128 keys, each with its own loads 131, 263, 58 (a block's
+// chain took 8,000 cycles, most of it its loads' latency at half of L2's rate); two tiles to a CTA and one warp that polls both
+// tiles' events 168, 299, 68 (1,100 to 1,700 cycles late); an MMA warp per tile 155, 285, 63 (both tiles keep step, so
+// both wait for their MMAs together); scores double buffered in blocks of 64: 100, 217, 58; items claimed, not dealt: 91, 208, 48. Slower
+// than this: two threads to a row (sixteen softmax warps: a cap -6 %, the others +5 to 10 %), the next block's scores loaded ahead of
+// this one's exponentials (+30 %), exponentials by polynomials on the FMA pipe for a half of them (+6 %), a delay to set the tiles out of step (0).
 // ---------------------------------------------------------------------------
 struct MaskedFwdParams {
   __nv_bfloat16* O;

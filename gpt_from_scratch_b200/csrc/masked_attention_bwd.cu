@@ -22,7 +22,7 @@ using gfs_host::strides_ok;
 namespace {
 
 // ---------------------------------------------------------------------------
-// Pre-pass: dvec[b, h, s] = sum_d dO * O, 0 for padding (whatever its dO holds) and for rows S .. S_pad. Eight threads per row,
+// Pre-pass (25 MB + 25 MB: 12 us): dvec[b, h, s] = sum_d dO * O, 0 for padding (whatever its dO holds) and for rows S .. S_pad. Eight threads per row,
 // 16 bytes (head_dim 128: twice) of each tensor, four rows a thread with all loads issued first; rows in the memory order of O
 // (heads or tokens fastest), one division by a constant of the launch per row.
 // ---------------------------------------------------------------------------
@@ -141,6 +141,16 @@ struct MBwdShape {
 // share the 32 rows of a quarter, 32 streamed columns each (no exchange is needed: the statistics are inputs). The
 // MMAs are issued by two warps (1: scores, 2: gradients), so neither order waits for the other. P / dS go to columns of their own
 // where there is room, for dK / dV at head_dim 128 to the columns of the scores they were made from.
+//
+// Bound, at head_dim 128, by shared memory feeding the tensor pipe: a score MMA of 128 x 64 x 16 reads 6 KB for 32 cycles of
+// multiplication, so that it takes 48, and with the gradients' a streamed tile needs 1,280 (dQ: 1,024) cycles of 1,790 (1,350); with
+// a cap by the chain of its 2.25 special function operations a score. us, dK / dV with dQ beside them (each alone): 16 heads (4
+// of k) of 8192 tokens, head_dim 128, documents with prefixes 232 (166, 114); 4 x 16 heads (4) of 2048, capped 181 (134, 89); 16 x 12
+// heads of 1024, head_dim 64, in documents of 200 tokens, four streamed tiles an item, 98 (62, 48): there items' ends weigh as much
+// as their tiles. What items cost was cut by a warp that prepares them (their plans, and the rows' statistics), by claiming them,
+// and by not parting groups of heads where there is an item for every SM (the first case 280 -> 232); not by loading the
+// next resident tiles early nor by prefetching rows into registers. Handing P over before dS is made, so that dV's products
+// start earlier, made registers spill: 146 -> 151 and 102 -> 162.
 template <int D, int MODE, bool CAP, bool DIST>
 __global__ void __launch_bounds__(MBWD_THREADS, 1)
 masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant__ CUtensorMap tr2,
@@ -641,10 +651,14 @@ masked_dkv_kernel(const float* partial, int parts, __nv_bfloat16* __restrict__ d
   }
 }
 
-// Into how many parts the heads of a group are dealt for dK and dV.
+// Into how many parts the heads of a group are dealt for dK and dV: until there is an item for every SM. Parts cost a pass over
+// fp32 sums; with more items than SMs the uneven end of this kernel is filled by dQ's, which starts beside it. us, forward
+// and backward, causal, 1 part -> 2 -> 4: [1, 32 heads (4), 2048, 128] (64 items) 333 -> ... -> 197, [1, 16 (1), 8192, 128] (64) 2511 -> ... ->
+// 1134, [1, 32 (4), 4096, 128] (128) 743 -> 612 -> 631, [1, 32 (8), 2048, 128] (128) 202 -> 202 -> 218; 256 items, [1, 32 (4), 8192, 128] 2205 ->
+// 2316 -> 2331, in documents [1, 16 (4), 8192, 128] 365 -> 395 -> 430.
 int group_parts(int tiles, int B, int nkv, int group) {
   int parts = 1;
-  while (parts < 4 && group % (2 * parts) == 0 && static_cast<long long>(tiles) * B * nkv * parts < 2ll * gfs_host::sm_count())
+  while (parts < 4 && group % (2 * parts) == 0 && static_cast<long long>(tiles) * B * nkv * parts < gfs_host::sm_count())
     parts *= 2;
   return tiles > 1 ? parts : 1;
 }
