@@ -300,7 +300,8 @@ __global__ void __launch_bounds__(MASK_THREADS) attention_mask_kernel(const Mask
 // 45 % of the time, with a cap (2.25 operations a score) for 75 %; the rest is the length of their chains. us, and
 // products at a share of the measured tensor rate: 16 heads (4 of k) of 8192 tokens, head_dim 128, documents with prefixes 91
 // (0.41); 64 heads (16 of k) of 4096 under a window of 1024, capped 208 (0.35); 16 x 12 heads of 1024 tokens of head_dim 64 in
-// documents of 200 tokens, where an item is five blocks and every fourth score is needed, 48 (100 MB: 15 at copy speed).
+// documents of 200 tokens, where an item is five blocks and every fourth score is needed, 48 (100 MB: 15 at copy speed). What the backward
+// needs is another half of the output: 8 more for the first and the last.
 //
 // What led here, us for the three: a CTA per tile, two per SM, blocks of 128 keys, each with its own loads 131, 263, 58 (a block's
 // chain took 8,000 cycles, most of it its loads' latency at half of L2's rate); two tiles to a CTA and one warp that polls both
@@ -313,6 +314,7 @@ struct MaskedFwdParams {
   __nv_bfloat16* O;
   long long o_ss, o_bs, o_hs;  // element strides: sequence, batch, head
   float* lse;                  // [B, nh, S_pad], base 2; +inf for rows that see nothing; or null
+  uint8_t* rest;               // with lse: [B, nh, S_pad, D], what O's rounding leaves out (bf16_rest)
   int S, S_pad, B, nh, group;
   int head_pairs;
   ScoreArgs score;
@@ -791,6 +793,16 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             ow[e] = seen ? pack_bf16x2(__uint_as_float(w[2 * e]) * inv, __uint_as_float(w[2 * e + 1]) * inv) : 0u;
+          if (p.lse != nullptr) {
+            uint32_t rest[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float o[4] = {__uint_as_float(w[4 * e]) * inv, __uint_as_float(w[4 * e + 1]) * inv,
+                                  __uint_as_float(w[4 * e + 2]) * inv, __uint_as_float(w[4 * e + 3]) * inv};
+              rest[e] = seen ? bf16_rest(o, ow[2 * e], ow[2 * e + 1]) : 0u;
+            }
+            st_global_256(p.rest + ((static_cast<size_t>(b) * p.nh + h) * p.S_pad + row) * D + cc * 32, rest);   // a sector
+          }
           store_rows_32x32(stage, ow, lane, g0 + cc * 32, p.o_ss, p.S - row0);
         }
         if (p.lse != nullptr)
@@ -864,14 +876,15 @@ void gfs_attention_mask_layout(int B, int S, long long* offsets) {
 }
 
 // q [B, nh, S, D], k and v [B, nkv, S, D], out like q; strides: 12 element strides {q, k, v, out} x {seq, batch, head}.
-// mask: from gfs_attention_mask, of the same B and S. lse: fp32 [B, nh, S_pad], base 2, or null (no backward will follow). cap 0: scores as they are.
+// mask: from gfs_attention_mask, of the same B and S. saved: for the backward, fp32 [B, nh, S_pad] (sums of exponentials, log base 2) and
+// behind them bytes [B, nh, S_pad, D] (what out's rounding leaves out), 32-byte aligned; or null. cap 0: scores as they are.
 // slopes: fp32 [nh] or null.
-int gfs_masked_attention_fwd(const void* q, const void* k, const void* v, void* out, void* lse, const void* mask, int S,
+int gfs_masked_attention_fwd(const void* q, const void* k, const void* v, void* out, void* saved, const void* mask, int S,
                              int B, int nh, int nkv, int D, const long long* strides, float scale, float cap,
                              const void* slopes, void* stream_) {
   if ((D != 64 && D != 128) || !strides_ok(strides, 12) || nkv <= 0 || nh % nkv != 0) return -1;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
-       reinterpret_cast<uintptr_t>(out)) & 15)
+       reinterpret_cast<uintptr_t>(out)) & 15 || reinterpret_cast<uintptr_t>(saved) & 31)
     return -2;
   if (S <= 0 || B <= 0 || nh <= 0) return 0;
   const int S_pad = (S + 127) / 128 * 128;
@@ -883,7 +896,8 @@ int gfs_masked_attention_fwd(const void* q, const void* k, const void* v, void* 
   MaskedFwdParams p;
   p.O = static_cast<__nv_bfloat16*>(out);
   p.o_ss = strides[9]; p.o_bs = strides[10]; p.o_hs = strides[11];
-  p.lse = static_cast<float*>(lse);
+  p.lse = static_cast<float*>(saved);
+  p.rest = saved == nullptr ? nullptr : static_cast<uint8_t*>(saved) + 4 * static_cast<size_t>(B) * nh * S_pad;
   p.S = S; p.S_pad = S_pad; p.B = B; p.nh = nh; p.group = nh / nkv;
   p.head_pairs = p.group % 2 == 0;
   p.score.sl2 = cap > 0.f ? 2.f * scale * LOG2E_F / cap : scale * LOG2E_F;

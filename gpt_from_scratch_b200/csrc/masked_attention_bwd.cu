@@ -22,13 +22,14 @@ using gfs_host::strides_ok;
 namespace {
 
 // ---------------------------------------------------------------------------
-// Pre-pass (25 MB + 25 MB: 12 us): dvec[b, h, s] = sum_d dO * O, 0 for padding (whatever its dO holds) and for rows S .. S_pad. Eight threads per row,
-// 16 bytes (head_dim 128: twice) of each tensor, four rows a thread with all loads issued first; rows in the memory order of O
+// Pre-pass (25 MB + 25 MB + 13 MB: 16 us): dvec[b, h, s] = sum_d dO * O, O with what its rounding left out, 0 for padding (whatever its dO
+// holds) and for rows S .. S_pad. Eight threads per row, 16 bytes (head_dim 128: twice) of each tensor, four rows a thread with all loads issued first; rows in the memory order of O
 // (heads or tokens fastest), one division by a constant of the launch per row.
 // ---------------------------------------------------------------------------
 constexpr int DVEC_ROWS = 4;
 struct DvecArgs {
   const __nv_bfloat16 *dO, *O;
+  const uint8_t* rest;         // [B, nh, S_pad, D]: what O's rounding left out
   float* dvec;
   const int *first, *last, *padded;
   int S, S_pad, nh;
@@ -46,6 +47,7 @@ __global__ void __launch_bounds__(256) masked_dvec_kernel(const DvecArgs a) {
   const unsigned total = static_cast<unsigned>(a.S_pad) * a.nh;
   const unsigned row0 = blockIdx.x * (32u * DVEC_ROWS) + (threadIdx.x >> 3);
   uint4 x[DVEC_ROWS][V], y[DVEC_ROWS][V];
+  uint2 z[DVEC_ROWS][V];
   unsigned at[DVEC_ROWS], token[DVEC_ROWS];
 #pragma unroll
   for (int i = 0; i < DVEC_ROWS; ++i) {
@@ -56,14 +58,19 @@ __global__ void __launch_bounds__(256) masked_dvec_kernel(const DvecArgs a) {
     at[i] = h * a.S_pad + s;
     token[i] = min(s, static_cast<unsigned>(a.S_pad) - 1u);
 #pragma unroll
-    for (int v = 0; v < V; ++v) x[i][v] = y[i][v] = make_uint4(0, 0, 0, 0);
+    for (int v = 0; v < V; ++v) {
+      x[i][v] = y[i][v] = make_uint4(0, 0, 0, 0);
+      z[i][v] = make_uint2(0, 0);
+    }
     if (row < total && s < static_cast<unsigned>(a.S)) {
       const __nv_bfloat16* px = a.dO + s * a.do_ss + b * a.do_bs + h * a.do_hs + sub * 8;
       const __nv_bfloat16* py = a.O + s * a.o_ss + b * a.o_bs + h * a.o_hs + sub * 8;
+      const uint8_t* pz = a.rest + (static_cast<size_t>(b) * a.nh * a.S_pad + at[i]) * D + sub * 8;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         x[i][v] = *reinterpret_cast<const uint4*>(px + 64 * v);
         y[i][v] = *reinterpret_cast<const uint4*>(py + 64 * v);
+        z[i][v] = *reinterpret_cast<const uint2*>(pz + 64 * v);
       }
     }
   }
@@ -77,7 +84,7 @@ __global__ void __launch_bounds__(256) masked_dvec_kernel(const DvecArgs a) {
       const uint32_t yw[4] = {y[i][v].x, y[i][v].y, y[i][v].z, y[i][v].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float2 a2 = unpack_bf16x2(xw[e]), b2 = unpack_bf16x2(yw[e]);
+        const float2 a2 = unpack_bf16x2(xw[e]), b2 = with_rest(yw[e], e < 2 ? z[i][v].x : z[i][v].y, 2 * (e & 1));
         acc += a2.x * b2.x + a2.y * b2.y;
       }
     }
@@ -705,14 +712,14 @@ long long gfs_masked_attention_scratch(int S, int B, int nh, int nkv, int D) {
 // size above; the rest as for gfs_masked_attention_fwd. dq shares no memory with anything that is read
 // for dk and dv, nor with them: its kernel runs beside theirs.
 int gfs_masked_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout,
-                             const void* lse, void* dvec, void* partial, void* dq, void* dk, void* dv,
+                             const void* saved, void* dvec, void* partial, void* dq, void* dk, void* dv,
                              const void* mask, int S, int B,
                              int nh, int nkv, int D, const long long* strides, float scale, float cap, const void* slopes,
                              void* stream_) {
   if ((D != 64 && D != 128) || !strides_ok(strides, 24) || nkv <= 0 || nh % nkv != 0) return -1;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
        reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(dq) |
-       reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15)
+       reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) | reinterpret_cast<uintptr_t>(saved)) & 15)
     return -2;
   if (S <= 0 || B <= 0 || nh <= 0) return 0;
   const int S_pad = (S + 127) / 128 * 128;
@@ -726,7 +733,8 @@ int gfs_masked_attention_bwd(const void* q, const void* k, const void* v, const 
   {
     const int s_fastest = so[0] < so[2] ? 1 : 0;
     const unsigned inner = s_fastest ? S_pad : nh, rows = static_cast<unsigned>(S_pad) * nh;
-    const DvecArgs a{static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out), static_cast<float*>(dvec),
+    const DvecArgs a{static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out),
+                     static_cast<const uint8_t*>(saved) + 4 * static_cast<size_t>(B) * nh * S_pad, static_cast<float*>(dvec),
                      p.mask.first, p.mask.last, p.mask.padded, S, S_pad, nh, sdo[0], sdo[1], sdo[2], so[0], so[1], so[2], inner,
                      rows + 32 * DVEC_ROWS < (1u << 24) && inner <= (1u << 16) ? (1ull << 40) / inner + 1 : 0ull, s_fastest};
     const dim3 grid((rows + 32 * DVEC_ROWS - 1) / (32 * DVEC_ROWS), B);
@@ -738,7 +746,7 @@ int gfs_masked_attention_bwd(const void* q, const void* k, const void* v, const 
                      make_map(q, D, S, nh, B, sq, 64), make_map(k, D, S, nkv, B, sk, 64),
                      make_map(v, D, S, nkv, B, sv, 64), make_map(dout, D, S, nh, B, sdo, 64)};
   if (!maps.q128 || !maps.k128 || !maps.v128 || !maps.do128 || !maps.q64 || !maps.k64 || !maps.v64 || !maps.do64) return -3;
-  p.lse = static_cast<const float*>(lse);
+  p.lse = static_cast<const float*>(saved);
   p.dvec = static_cast<const float*>(dvec);
   p.S = S; p.S_pad = S_pad; p.B = B; p.nh = nh; p.group = nh / nkv; p.scale = scale;
   p.score.sl2 = cap > 0.f ? 2.f * scale * LOG2E_F / cap : scale * LOG2E_F;

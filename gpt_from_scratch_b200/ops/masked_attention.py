@@ -174,18 +174,19 @@ def _readable(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _forward(q, k, v, buffer, slopes, softcap: float, scale: float, want_lse: bool):
+def _forward(q, k, v, buffer, slopes, softcap: float, scale: float, training: bool):
     B, nh, S, D = q.shape
     out = torch.empty_like(q)
-    lse = torch.empty((B, nh, _pad128(S)), dtype=torch.float32, device=q.device) if want_lse else None
+    # for the backward: 32 bits per row (the log of its sum) and 8 bits per number (what rounding leaves out of ``out``)
+    saved = torch.empty(B * nh * _pad128(S) * (1 + D // 4), dtype=torch.float32, device=q.device) if training else None
     kv = k.shape
     st = _stride_array(q.shape, q.stride(), kv, k.stride(), kv, v.stride(), q.shape, out.stride())
     with _lib.on_device(q), _lib.nvtx("masked_attention_fwd"):
-        rc = _lib.lib().gfs_masked_attention_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _lib.ptr(lse),
+        rc = _lib.lib().gfs_masked_attention_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _lib.ptr(saved),
                                                  buffer.data_ptr(), S, B, nh, kv[1], D, st, scale, softcap,
                                                  _lib.ptr(slopes), _lib.stream_ptr())
     _lib.check(rc, "gfs_masked_attention_fwd")
-    return out, lse
+    return out, saved
 
 
 @functools.lru_cache(maxsize=256)
@@ -197,15 +198,15 @@ class _MaskedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, buffer, slopes, softcap, scale):
         q, k, v = _readable(q), _readable(k), _readable(v)
-        out, lse = _forward(q, k, v, buffer, slopes, softcap, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, buffer, slopes)
+        out, saved = _forward(q, k, v, buffer, slopes, softcap, scale, True)
+        ctx.save_for_backward(q, k, v, out, saved, buffer, slopes)
         ctx.args = (softcap, scale)
         return out
 
     @staticmethod
     @_lib.first_order
     def backward(ctx, dout):
-        q, k, v, out, lse, buffer, slopes = ctx.saved_tensors
+        q, k, v, out, saved, buffer, slopes = ctx.saved_tensors
         softcap, scale = ctx.args
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         if q.numel() == 0:
@@ -213,14 +214,14 @@ class _MaskedAttention(torch.autograd.Function):
         B, nh, S, D = shape = q.shape
         kv = k.shape
         dout = _readable(dout)
-        dvec = torch.empty_like(lse)
+        dvec = torch.empty(B * nh * _pad128(S), dtype=torch.float32, device=q.device)
         scratch = _scratch(S, B, nh, kv[1], D)
         partial = torch.empty(scratch, dtype=torch.float32, device=q.device) if scratch else None
         st = _stride_array(shape, q.stride(), kv, k.stride(), kv, v.stride(), shape, out.stride(), shape, dout.stride(), shape,
                            dq.stride(), kv, dk.stride(), kv, dv.stride())
         with _lib.on_device(q), _lib.nvtx("masked_attention_bwd"):
             rc = _lib.lib().gfs_masked_attention_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                                     dout.data_ptr(), lse.data_ptr(), dvec.data_ptr(), _lib.ptr(partial),
+                                                     dout.data_ptr(), saved.data_ptr(), dvec.data_ptr(), _lib.ptr(partial),
                                                      dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), buffer.data_ptr(), S, B,
                                                      nh, kv[1], D, st, scale, softcap, _lib.ptr(slopes), _lib.stream_ptr())
         _lib.check(rc, "gfs_masked_attention_bwd")

@@ -6,7 +6,7 @@ terms with scores up to ~ 60, the exponential, the capped score to ~ 2^-18) chan
 
   |dout|  <= u |out| + (u + f) p |v|                                   =: u |out| + A
   |ddV|   <= u |dV| + (u + f) p' |dO|
-  dvec    = rowsum(dO * out) of the rounded out: off by E = |dO| (u |out| + A)
+  dvec    = rowsum(dO * out): off by E = |dO| (u |out| + A) (out is saved more precisely than it is rounded: less than this)
   |ddQ|   <= u |dQ| + scale ((u + f) |dS| + p g (E + 2^-14 (|dP| + |dvec|))) |k|      g: derivative of the capped score
   |ddK|   <= the same with the transposed matrix and |q|
 
@@ -401,3 +401,37 @@ def test_positions_norm_rotation_and_attention_together(cuda_device):
         assert torch.isfinite(a).all() and (a.double() - b).norm() <= 2.0 ** -6 * b.norm()
     pad = (ids < 0).t()
     assert (got[0][pad] == 0).all() and (got[1][pad] == 0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_gradients_of_scores_do_not_see_the_rounding_of_outputs(D):
+    """Documents of two tokens with one key twice and values a few steps apart: the second query's output lies between two bf16 numbers, and
+    its gradients are what differs between the values."""
+    B, H, S = 2, 2, 82
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    q, k, dout = (torch.randn(B, H, S, D, device="cuda", generator=gen).bfloat16() for _ in range(3))
+    k[:, :, 1::2] = k[:, :, 0::2]
+    steps = torch.randint(1, 100, (B, H, S, D), device="cuda", generator=gen)
+    steps[:, :, 1::2] = steps[:, :, 0::2] + torch.randint(-3, 4, (B, H, S // 2, D), device="cuda", generator=gen)
+    v = (1.0 + steps * 2.0 ** -7).bfloat16()                       # in [1, 2), where a step is 2^-7
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    ids = (torch.arange(S, device="cuda") // 2).int().expand(B, S)
+    out = ops.masked_attention(q, k, v, ops.attention_mask(B, S, document_ids=ids))
+    dk, = torch.autograd.grad(out, k, dout)
+
+    first, second = slice(0, None, 2), slice(1, None, 2)
+    q64, v64, do64 = (t.detach().double() for t in (q, v, dout))
+    ds = 0.25 * (do64[:, :, second] * (v64[:, :, first] - v64[:, :, second])).sum(-1, keepdim=True)
+    want = torch.zeros_like(q64)
+    want[:, :, first], want[:, :, second] = ds * q64[:, :, second] / D ** 0.5, -ds * q64[:, :, second] / D ** 0.5
+    # dS and dk are rounded to bf16 once each, P = 1/2 is recomputed to less than 2^-15. dP - dvec, of which dS is half: outputs of 1 to 2
+    # are saved to 2^-8 of a step of 2^-7 (2^-16 of `size`), and both are sums of D products in 32 bits
+    size = (do64.abs() * 2.0).sum(-1, keepdim=True)
+    off = 0.5 * size * (2.0 ** -16 + 2 * D * 2.0 ** -24)
+    off = off[:, :, second] * q64[:, :, second].abs() / D ** 0.5
+    bound = want.abs() * (2 * 2.0 ** -8 + 2.0 ** -15)
+    for part in (first, second):
+        bound[:, :, part] += off * (1 + 2 * 2.0 ** -8)
+    # the first query sees its own key alone: dP - dvec is the sums' rounding
+    bound[:, :, first] += size[:, :, first] * 2 * D * 2.0 ** -24 * q64[:, :, first].abs() / D ** 0.5
+    assert ((dk.double() - want).abs() <= bound).all()
