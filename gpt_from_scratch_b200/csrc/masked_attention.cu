@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(MASK_THREADS) attention_mask_kernel(const Mask
   const int b = blockIdx.x;
   const size_t row = static_cast<size_t>(b) * a.S;
   const size_t prow = static_cast<size_t>(b) * a.S_pad;
-  const int chunks = (a.S_pad + MASK_THREADS * N - 1) / (MASK_THREADS * N);      // (S_pad < 2^31 - 2^13: S is checked)
+  const int chunks = (a.S_pad + MASK_THREADS * N - 1) / (MASK_THREADS * N);      // (i0 + N fits an int: S is checked)
   // what a thread's tokens hold: the first of a document, prefix, padding (bits)
   struct Tokens {
     unsigned starts, prefix, pad;
@@ -853,7 +853,7 @@ extern "C" {
 // aligned.
 int gfs_attention_mask(const void* ids, int ids64, const void* prefix, int B, int S, int causal, int window, void* out,
                        void* stream) {
-  if (S < 0 || B < 0 || window < 0 || (!causal && (window > 0 || prefix != nullptr)) || S > 0x7fff0000) return -1;
+  if (S < 0 || B < 0 || window < 0 || (!causal && (window > 0 || prefix != nullptr)) || S > 0x3fff0000) return -1;   // (i + window fits an int)
   if (S == 0 || B == 0) return 0;
   if (reinterpret_cast<uintptr_t>(out) & 15) return -2;
   int* o = static_cast<int*>(out);

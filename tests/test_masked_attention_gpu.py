@@ -404,7 +404,7 @@ def test_positions_norm_rotation_and_attention_together(cuda_device):
 
 
 @pytest.mark.parametrize("D", [64, 128])
-def test_gradients_of_scores_do_not_see_the_rounding_of_outputs(D):
+def test_gradients_of_scores_do_not_see_the_rounding_of_outputs(cuda_device, D):
     """Documents of two tokens with one key twice and values a few steps apart: the second query's output lies between two bf16 numbers, and
     its gradients are what differs between the values."""
     B, H, S = 2, 2, 82
@@ -435,3 +435,26 @@ def test_gradients_of_scores_do_not_see_the_rounding_of_outputs(D):
     # the first query sees its own key alone: dP - dvec is the sums' rounding
     bound[:, :, first] += size[:, :, first] * 2 * D * 2.0 ** -24 * q64[:, :, first].abs() / D ** 0.5
     assert ((dk.double() - want).abs() <= bound).all()
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """2.25e9 numbers in q and all that is like it; the last queries and keys are looked at."""
+    B, nh, S, D, window, tail = 1, 16, 1_100_000, 128, 64, 512
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q, dout = (torch.empty(B, nh, S, D, device="cuda", dtype=torch.bfloat16).normal_(generator=gen) for _ in range(2))
+    k, v = (torch.empty(B, 1, S, D, device="cuda", dtype=torch.bfloat16).normal_(generator=gen) for _ in range(2))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = ops.masked_attention(*leaves, ops.attention_mask(B, S, window=window, device="cuda"))
+    grads = torch.autograd.grad(out, leaves, dout)
+    at = torch.arange(tail, device="cuda")
+    see = ((at[:, None] >= at) & (at > at[:, None] - window)).expand(B, tail, tail)
+    wants, tols = bounds_and_values(*(t[:, :, -tail:] for t in (q, k, v, dout)), see, 0.0, None, D ** -0.5)
+    for got, want, tol in zip((out, *grads), wants, tols):       # (the tail's first queries see keys before it)
+        assert ((got[:, :, -tail:].double() - want).abs() <= tol)[:, :, window:].all()
+    del out, grads, dout
+
+    x = q.detach().view(S, B, nh, D)
+    cos, sin = ops.rope_tables(S, D, device="cuda")
+    want = ops.rotary_reference(x[-tail:].double(), cos[-tail:].double(), sin[-tail:].double())
+    off = (ops.rotary(x, cos, sin)[-tail:].double() - want).abs()
+    assert (off <= U * want.abs() + 2.0 ** -22 * x[-tail:].double().abs().amax()).all()
