@@ -22,11 +22,12 @@ using gfs_host::strides_ok;
 namespace {
 
 // ---------------------------------------------------------------------------
-// Pre-pass (25 MB + 25 MB + 13 MB: 16 us): dvec[b, h, s] = sum_d dO * O, O with what its rounding left out, 0 for padding (whatever its dO
-// holds) and for rows S .. S_pad. Eight threads per row, 16 bytes (head_dim 128: twice) of each tensor, four rows a thread with all loads issued first; rows in the memory order of O
-// (heads or tokens fastest), one division by a constant of the launch per row.
+// Pre-pass (25 MB + 25 MB + 13 MB: 16 us): dvec[b, h, s] = sum_d dO * O, O with what its rounding left out, 0 for padding (whatever its
+// dO holds) and for rows S .. S_pad. Eight threads per row, 16 bytes (head_dim 128: twice) of dO and O, four rows (two: four leave
+// room for two CTAs per SM, 4 us more) a thread with all loads issued first; rows in the memory order of O (heads or tokens
+// fastest), one division by a constant of the launch per row.
 // ---------------------------------------------------------------------------
-constexpr int DVEC_ROWS = 4;
+constexpr int dvec_rows(int D) { return 256 / D; }
 struct DvecArgs {
   const __nv_bfloat16 *dO, *O;
   const uint8_t* rest;         // [B, nh, S_pad, D]: what O's rounding left out
@@ -43,14 +44,15 @@ __global__ void __launch_bounds__(256) masked_dvec_kernel(const DvecArgs a) {
   pdl_wait();
   pdl_trigger();
   constexpr int V = D / 64;                     // 16-byte vectors a thread
+  constexpr int ROWS = dvec_rows(D);
   const int sub = threadIdx.x & 7, b = blockIdx.y;
   const unsigned total = static_cast<unsigned>(a.S_pad) * a.nh;
-  const unsigned row0 = blockIdx.x * (32u * DVEC_ROWS) + (threadIdx.x >> 3);
-  uint4 x[DVEC_ROWS][V], y[DVEC_ROWS][V];
-  uint2 z[DVEC_ROWS][V];
-  unsigned at[DVEC_ROWS], token[DVEC_ROWS];
+  const unsigned row0 = blockIdx.x * (32u * ROWS) + (threadIdx.x >> 3);
+  uint4 x[ROWS][V], y[ROWS][V];
+  uint2 z[ROWS][V];
+  unsigned at[ROWS], token[ROWS];
 #pragma unroll
-  for (int i = 0; i < DVEC_ROWS; ++i) {
+  for (int i = 0; i < ROWS; ++i) {
     const unsigned row = row0 + 32u * i;
     const unsigned outer = a.magic != 0 ? static_cast<unsigned>((row * a.magic) >> 40) : row / a.inner;
     const unsigned rest = row - outer * a.inner;
@@ -76,7 +78,7 @@ __global__ void __launch_bounds__(256) masked_dvec_kernel(const DvecArgs a) {
   }
   const bool padded = a.padded[b] != 0;       // (after the loads: they do not wait for it)
 #pragma unroll
-  for (int i = 0; i < DVEC_ROWS; ++i) {
+  for (int i = 0; i < ROWS; ++i) {
     float acc = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -733,11 +735,12 @@ int gfs_masked_attention_bwd(const void* q, const void* k, const void* v, const 
   {
     const int s_fastest = so[0] < so[2] ? 1 : 0;
     const unsigned inner = s_fastest ? S_pad : nh, rows = static_cast<unsigned>(S_pad) * nh;
+    const unsigned per_block = 32 * dvec_rows(D);
     const DvecArgs a{static_cast<const __nv_bfloat16*>(dout), static_cast<const __nv_bfloat16*>(out),
                      static_cast<const uint8_t*>(saved) + 4 * static_cast<size_t>(B) * nh * S_pad, static_cast<float*>(dvec),
                      p.mask.first, p.mask.last, p.mask.padded, S, S_pad, nh, sdo[0], sdo[1], sdo[2], so[0], so[1], so[2], inner,
-                     rows + 32 * DVEC_ROWS < (1u << 24) && inner <= (1u << 16) ? (1ull << 40) / inner + 1 : 0ull, s_fastest};
-    const dim3 grid((rows + 32 * DVEC_ROWS - 1) / (32 * DVEC_ROWS), B);
+                     rows + per_block < (1u << 24) && inner <= (1u << 16) ? (1ull << 40) / inner + 1 : 0ull, s_fastest};
+    const dim3 grid((rows + per_block - 1) / per_block, B);
     gfs_host::launch_pdl(D == 64 ? masked_dvec_kernel<64> : masked_dvec_kernel<128>, grid, dim3(256), 0, stream, a);
     if (cudaGetLastError() != cudaSuccess) return -11;
   }
