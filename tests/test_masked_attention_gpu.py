@@ -4,7 +4,9 @@ Tolerances, derived beforehand. u = 2^-8 is half a step of bf16. Probabilities a
 dO (u, relative), a result is rounded once more (u of the result), and what fp32 does before that (dot products of up to 128
 terms with scores up to ~ 60, the exponential, the capped score to ~ 2^-18) changes a probability by less than f = 2^-12, relative:
 
-  |dout|  <= u |out| + (u + f) p |v|                                   =: u |out| + A
+  |dout|  <= u |out| + (u + f) p |v| + u |out|                         =: u |out| + A
+             (out = sum_j P_j v_j / sum_j P_j of the rounded P_j = p_j (1 + e_j), |e_j| <= u: off by sum_j p_j e_j (v_j - out), and
+             sum_j p_j |v_j - out| <= p |v| + |out|, nearly reached where two keys are seen)
   |ddV|   <= u |dV| + (u + f) p' |dO|
   dvec    = rowsum(dO * out): off by E = |dO| (u |out| + A) (out is saved more precisely than it is rounded: less than this)
   |ddQ|   <= u |dQ| + scale ((u + f) |dS| + p g (E + 2^-14 (|dP| + |dvec|))) |k|      g: derivative of the capped score
@@ -44,7 +46,7 @@ def bounds_and_values(q, k, v, dout, see, softcap, slopes, scale):
     p = torch.exp(s - top)
     p = p / p.sum(-1, keepdim=True).clamp_min(1e-300)
     out = p @ vv
-    A = (U + F) * (p @ vv.abs())
+    A = (U + F) * (p @ vv.abs()) + U * out.abs()
     tol_out = U * out.abs() + A
     dP = do @ vv.transpose(-1, -2)
     dvec = (do * out).sum(-1, keepdim=True)
@@ -168,6 +170,7 @@ FORMS = [
     (8, 12, 12, 130, 64, "docs", True, False, None, 0.0, False),
     (1, 16, 16, 1500, 64, "padded", True, False, 300, 0.0, False),
     (2, 20, 4, 900, 128, "docs", True, True, None, 0.0, False),
+    (1, 32, 8, 252, 128, "none", True, False, 2, 5.0, False),
 ]
 
 
