@@ -301,18 +301,17 @@ __global__ void __launch_bounds__(MASK_THREADS) attention_mask_kernel(const Mask
 // products at a share of the measured tensor rate: 16 heads (4 of k) of 8192 tokens, head_dim 128, documents with prefixes 91
 // (0.41); 64 heads (16 of k) of 4096 under a window of 1024, capped 208 (0.35); 16 x 12 heads of 1024 tokens of head_dim 64 in
 // documents of 200 tokens, where an item is five blocks and every fourth score is needed, 48 (100 MB: 15 at copy speed). What the backward
-// needs is another half of the output: 8 more for the first and the last.
+// needs is another half of the output: 5 to 8 more for the first and the last.
 //
 // What led here, us for the three: a CTA per tile, two per SM, blocks of 128 keys, each with its own loads 131, 263, 58 (a block's
 // chain took 8,000 cycles, most of it its loads' latency at half of L2's rate); two tiles to a CTA and one warp that polls both
 // tiles' events 168, 299, 68 (1,100 to 1,700 cycles late); an MMA warp per tile 155, 285, 63 (both tiles keep step, so
 // both wait for their MMAs together); scores double buffered in blocks of 64: 100, 217, 58; items claimed, not dealt: 91, 208, 48. Slower
 // than this: two threads to a row (sixteen softmax warps: a cap -6 %, the others +5 to 10 %), the next block's scores loaded ahead of
-// this one's exponentials (+30 %), exponentials by polynomials on the FMA pipe for a half of them (+6 %), a delay to set the tiles out of step (0).
+// this one's exponentials (+30 %), exponentials by polynomials on the FMA pipe for a half of them (+6 %), a delay to set the tiles out of step (0), four more warps
+// that put the outputs out (+4 to 9 %), blocks classed by 32 rows and 32 keys, with no exponentials where nothing is seen (0 to +5 %).
 // ---------------------------------------------------------------------------
 struct MaskedFwdParams {
-  __nv_bfloat16* O;
-  long long o_ss, o_bs, o_hs;  // element strides: sequence, batch, head
   float* lse;                  // [B, nh, S_pad], base 2; +inf for rows that see nothing; or null
   uint8_t* rest;               // with lse: [B, nh, S_pad, D], what O's rounding leaves out (bf16_rest)
   int S, S_pad, B, nh, group;
@@ -343,7 +342,7 @@ struct MFwdShape {
   static constexpr int DB = D / 64;
   static constexpr int Q_TILE = DB * 16384, KV_TILE = DB * 8192;    // 128 queries, 64 keys
   static constexpr int KS = D == 64 ? 8 : 4;        // stages of K and V
-  static constexpr int STAGING = MFWD_SW * 2048;    // to transpose the output rows through
+  static constexpr int STAGING = MFWD_SW * 4096;    // a warp's results on their way out: 32 rows of 64 columns
   static constexpr int SMEM = 2 * Q_TILE + 2 * KS * KV_TILE + STAGING + sizeof(FwdItem) + 512;
 };
 // Scores: as they are, capped with a bound that the running maximum may be left out for, capped.
@@ -355,7 +354,8 @@ constexpr float BOUNDED_CAP2 = 80.f;
 template <int D, int SCORES, bool DIST>
 __global__ void __launch_bounds__(MFWD_THREADS, 1)
 masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                  const __grid_constant__ CUtensorMap tv, const MaskedFwdParams p, int n_levels) {
+                  const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to, const MaskedFwdParams p,
+                  int n_levels) {
   using Shape = MFwdShape<D>;
   constexpr int DB = Shape::DB, Q_TILE = Shape::Q_TILE, KV_TILE = Shape::KV_TILE, KS = Shape::KS;
   constexpr uint32_t O_COL = 256;            // scores at [tile][buffer][64] before that; P takes the columns of its scores
@@ -410,6 +410,7 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
     tma_prefetch_desc(&tq);
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
+    tma_prefetch_desc(&to);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -622,7 +623,7 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_base + x * 128;
     const uint32_t o_addr = tmem_base + lane_base + O_COL + x * D;
-    uint8_t* stage = staging + (warp - MFWD_FIRST_SW) * 2048;
+    uint8_t* stage = staging + (warp - MFWD_FIRST_SW) * 4096;
     constexpr bool MAXED = SCORES != BOUNDED;
     const float sl2 = p.score.sl2, cap2 = p.score.cap2;
     const float k = SCORES != PLAIN || DIST ? 1.f : sl2;    // what turns the numbers in the registers into exponents
@@ -778,11 +779,16 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
         const int c_last = cdone + j1 - j0 - 1;
         mbar_wait(&o_full[2 * x + (c_last & 1)], (c_last >> 1) & 1, wctx, STATUS_TIMEOUT_SOFTMAX);
         tc_fence_after();
+        // Rows leave by TMA: a warp that stores them itself waits for its SM's share of the write rate (whole calls, us: 64 heads of
+        // 4096 under a window 225 -> 219, 8192 tokens with prefixes 373 -> 368; what the backward needs is faster stored directly, 174 -> 170 for documents).
         const int row0 = row - lane;
-        __nv_bfloat16* g0 = p.O + row0 * p.o_ss + b * p.o_bs + h * p.o_hs;
 #pragma unroll
         for (int cc = 0; cc < D / 32; ++cc) {
           uint32_t w[32], ow[16];
+          if (cc % 2 == 0) {         // what was there has left
+            if (lane == 0) bulk_wait_read_all();
+            __syncwarp();
+          }
           tmem_ld_32x32(o_addr + cc * 32, w);
           tmem_ld_wait_for(w);
           if (cc == D / 32 - 1) {    // the next item's first P V may overwrite the accumulator
@@ -803,7 +809,18 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
             }
             st_global_256(p.rest + ((static_cast<size_t>(b) * p.nh + h) * p.S_pad + row) * D + cc * 32, rest);   // a sector
           }
-          store_rows_32x32(stage, ow, lane, g0 + cc * 32, p.o_ss, p.S - row0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((((cc & 1) * 4 + i) ^ (lane & 7)) << 4)) =
+                make_uint4(ow[4 * i], ow[4 * i + 1], ow[4 * i + 2], ow[4 * i + 3]);
+          if (cc & 1) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && row0 < p.S) {        // (rows past the last token are cut off)
+              tma_store_4d(&to, stage, (cc - 1) * 32, row0, h, b);
+              bulk_commit();
+            }
+          }
         }
         if (p.lse != nullptr)
           p.lse[(static_cast<size_t>(b) * p.nh + h) * p.S_pad + row] =
@@ -811,6 +828,7 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
       }
       cdone += j1 - j0;
     }
+    if (lane == 0) bulk_wait_all();
   }
 
   tc_fence_before();
@@ -819,27 +837,29 @@ masked_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant_
   if (warp == 1) tmem_dealloc(tmem_base, 512);
 }
 
+struct FwdMaps {
+  const CUtensorMap *q, *k, *v, *o;
+};
+
 template <int D, int SCORES, bool DIST>
-int launch_fwd(const CUtensorMap* tq, const CUtensorMap* tk, const CUtensorMap* tv, const MaskedFwdParams& p,
-               cudaStream_t stream) {
+int launch_fwd(const FwdMaps& m, const MaskedFwdParams& p, cudaStream_t stream) {
   static gfs_host::SmemLimit limit;
   constexpr int smem = MFwdShape<D>::SMEM;
   if (!limit.raise(masked_fwd_kernel<D, SCORES, DIST>, smem)) return -10;
   const int tiles = p.S_pad / 128;
   const int n_levels = p.head_pairs ? tiles : (tiles + 1) / 2;
   const unsigned n_items = static_cast<unsigned>(n_levels) * p.B * (p.head_pairs ? p.nh / 2 : p.nh);
-  gfs_host::launch_pdl(masked_fwd_kernel<D, SCORES, DIST>, dim3(n_items), dim3(MFWD_THREADS), smem, stream, *tq, *tk,
-                       *tv, p, n_levels);
+  gfs_host::launch_pdl(masked_fwd_kernel<D, SCORES, DIST>, dim3(n_items), dim3(MFWD_THREADS), smem, stream, *m.q,
+                       *m.k, *m.v, *m.o, p, n_levels);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 template <int D, bool DIST>
-int launch_fwd_scores(const CUtensorMap* tq, const CUtensorMap* tk, const CUtensorMap* tv, const MaskedFwdParams& p,
-                      cudaStream_t stream) {
-  if (p.score.cap2 <= 0.f) return launch_fwd<D, PLAIN, DIST>(tq, tk, tv, p, stream);
+int launch_fwd_scores(const FwdMaps& m, const MaskedFwdParams& p, cudaStream_t stream) {
+  if (p.score.cap2 <= 0.f) return launch_fwd<D, PLAIN, DIST>(m, p, stream);
   if constexpr (!DIST) {       // a bias has no bound: a slope may be negative
-    if (p.score.cap2 <= BOUNDED_CAP2) return launch_fwd<D, BOUNDED, false>(tq, tk, tv, p, stream);
+    if (p.score.cap2 <= BOUNDED_CAP2) return launch_fwd<D, BOUNDED, false>(m, p, stream);
   }
-  return launch_fwd<D, CAPPED, DIST>(tq, tk, tv, p, stream);
+  return launch_fwd<D, CAPPED, DIST>(m, p, stream);
 }
 
 }  // namespace
@@ -889,13 +909,10 @@ int gfs_masked_attention_fwd(const void* q, const void* k, const void* v, void* 
   if (S <= 0 || B <= 0 || nh <= 0) return 0;
   const int S_pad = (S + 127) / 128 * 128;
   if (static_cast<long long>(S_pad / 128) * B * nh > 0x7fffffffll) return -1;
-  const CUtensorMap* tq = make_map(q, D, S, nh, B, strides + 0, 128);
-  const CUtensorMap* tk = make_map(k, D, S, nkv, B, strides + 3, 64);
-  const CUtensorMap* tv = make_map(v, D, S, nkv, B, strides + 6, 64);
-  if (!tq || !tk || !tv) return -3;
+  const FwdMaps m{make_map(q, D, S, nh, B, strides + 0, 128), make_map(k, D, S, nkv, B, strides + 3, 64),
+                  make_map(v, D, S, nkv, B, strides + 6, 64), make_map(out, D, S, nh, B, strides + 9, 32)};
+  if (!m.q || !m.k || !m.v || !m.o) return -3;
   MaskedFwdParams p;
-  p.O = static_cast<__nv_bfloat16*>(out);
-  p.o_ss = strides[9]; p.o_bs = strides[10]; p.o_hs = strides[11];
   p.lse = static_cast<float*>(saved);
   p.rest = saved == nullptr ? nullptr : static_cast<uint8_t*>(saved) + 4 * static_cast<size_t>(B) * nh * S_pad;
   p.S = S; p.S_pad = S_pad; p.B = B; p.nh = nh; p.group = nh / nkv;
@@ -907,8 +924,8 @@ int gfs_masked_attention_fwd(const void* q, const void* k, const void* v, void* 
   p.status = gfs_host::status_words();
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (slopes != nullptr)
-    return D == 64 ? launch_fwd_scores<64, true>(tq, tk, tv, p, stream) : launch_fwd_scores<128, true>(tq, tk, tv, p, stream);
-  return D == 64 ? launch_fwd_scores<64, false>(tq, tk, tv, p, stream) : launch_fwd_scores<128, false>(tq, tk, tv, p, stream);
+    return D == 64 ? launch_fwd_scores<64, true>(m, p, stream) : launch_fwd_scores<128, true>(m, p, stream);
+  return D == 64 ? launch_fwd_scores<64, false>(m, p, stream) : launch_fwd_scores<128, false>(m, p, stream);
 }
 
 }  // extern "C"
