@@ -105,13 +105,14 @@ __device__ __forceinline__ void store_rows_32x64(uint8_t* stage, const uint32_t 
 
 namespace gfs_host {
 
-inline const CUtensorMap* make_map(const void* base, int D, int S, int nh, int B, const long long* st, uint32_t box_rows) {
+inline const CUtensorMap* make_map(const void* base, int D, int S, int nh, int B, const long long* st, uint32_t box_rows,
+                                  uint32_t box_cols = 64) {
   // st = {seq, batch, head} element strides
   uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(S), static_cast<uint64_t>(nh),
                       static_cast<uint64_t>(B)};
   uint64_t strides[4] = {2, static_cast<uint64_t>(st[0]) * 2, static_cast<uint64_t>(st[2]) * 2,
                          static_cast<uint64_t>(st[1]) * 2};
-  uint32_t box[4] = {64, box_rows, 1, 1};
+  uint32_t box[4] = {box_cols, box_rows, 1, 1};
   return tmap_nd_cached(base, 4, dims, strides, box);
 }
 

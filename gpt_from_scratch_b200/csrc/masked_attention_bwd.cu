@@ -102,12 +102,8 @@ __global__ void __launch_bounds__(256) masked_dvec_kernel(const DvecArgs a) {
 // Main kernel
 // ---------------------------------------------------------------------------
 struct MaskedBwdParams {
-  __nv_bfloat16* out1;  // mode 0: dK, mode 1: dQ
-  __nv_bfloat16* out2;  // mode 0: dV
   float* partial;       // mode 0, parts > 1: fp32 [parts][dK, dV][B, nkv, S_pad, D]
   int parts;            // the heads of a group are dealt to this many items
-  long long o1_ss, o1_bs, o1_hs;
-  long long o2_ss, o2_bs, o2_hs;
   const float* lse;   // [B, nh, S_pad], base 2
   const float* dvec;  // [B, nh, S_pad]
   int S, S_pad, B, nh, group;
@@ -157,13 +153,15 @@ struct MBwdShape {
 // of k) of 8192 tokens, head_dim 128, documents with prefixes 232 (166, 114); 4 x 16 heads (4) of 2048, capped 181 (134, 89); 16 x 12
 // heads of 1024, head_dim 64, in documents of 200 tokens, four streamed tiles an item, 98 (62, 48): there items' ends weigh as much
 // as their tiles. What items cost was cut by a warp that prepares them (their plans, and the rows' statistics), by claiming them,
-// and by not parting groups of heads where there is an item for every SM (the first case 280 -> 232); not by loading the
+// by not parting groups of heads where there is an item for every SM (the first case 280 -> 232), and by results that leave by TMA
+// (whole calls 368 -> 362, 284 -> 279, 170 -> 166); not by loading the
 // next resident tiles early nor by prefetching rows into registers. Handing P over before dS is made, so that dV's products
 // start earlier, made registers spill: 146 -> 151 and 102 -> 162.
 template <int D, int MODE, bool CAP, bool DIST>
 __global__ void __launch_bounds__(MBWD_THREADS, 1)
 masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant__ CUtensorMap tr2,
                   const __grid_constant__ CUtensorMap tt1, const __grid_constant__ CUtensorMap tt2,
+                  const __grid_constant__ CUtensorMap to1, const __grid_constant__ CUtensorMap to2,     // mode 0: dK, dV; mode 1: dQ, -
                   const MaskedBwdParams p, int n_rt) {
   using Shape = MBwdShape<D, MODE>;
   constexpr int DB = D / 64;
@@ -240,6 +238,8 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
     tma_prefetch_desc(&tr2);
     tma_prefetch_desc(&tt1);
     tma_prefetch_desc(&tt2);
+    tma_prefetch_desc(&to1);
+    if (MODE == 0) tma_prefetch_desc(&to2);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, TMEM_COLS);
@@ -577,9 +577,6 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
       const int c0 = (MODE == 0) ? half * (D / 2) : (D == 128 ? group * 64 + half * 32 : half * 32);
       const bool is_dv = MODE == 0 && group == 1;
       const float out_scale = is_dv ? 1.f : (CAP ? 4.f : 1.f) * p.scale;
-      const long long o_ss = is_dv ? p.o2_ss : p.o1_ss;
-      __nv_bfloat16* out = is_dv ? p.out2 + row0 * p.o2_ss + b * p.o2_bs + h * p.o2_hs
-                                 : p.out1 + row0 * p.o1_ss + b * p.o1_bs + h * p.o1_hs;
       const uint32_t acc = tmem_base + lane_base + (MODE == 0 && !is_dv ? ACC2 : ACC1);
 #pragma unroll
       for (int ci = 0; ci < NC; ++ci) {
@@ -618,12 +615,24 @@ masked_bwd_kernel(const __grid_constant__ CUtensorMap tr1, const __grid_constant
             const float2 o = unpack_f32x2(mul_f32x2(pack_u32x2(v[2 * e], v[2 * e + 1]), scale2));
             wv[e] = pack_bf16x2(o.x, o.y);
           }
-          store_rows_32x32(stage, wv, lane, out + c, o_ss, p.S - row0);
+          if (lane == 0) bulk_wait_read_all();       // what was staged there has left
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(wv[4 * i], wv[4 * i + 1], wv[4 * i + 2], wv[4 * i + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && row0 < p.S) {             // (rows past the last token are cut off)
+            tma_store_4d(is_dv ? &to2 : &to1, stage, c, row0, h, b);
+            bulk_commit();
+          }
         }
       }
     }
   }
 
+  if (warp >= MBWD_FIRST_CW && lane == 0) bulk_wait_all();
   if (MODE == 1) pdl_wait();
   tc_fence_before();
   __syncthreads();
@@ -673,7 +682,7 @@ int group_parts(int tiles, int B, int nkv, int group) {
 }
 
 struct BwdMaps {
-  const CUtensorMap *q128, *k128, *v128, *do128, *q64, *k64, *v64, *do64;
+  const CUtensorMap *q128, *k128, *v128, *do128, *q64, *k64, *v64, *do64, *dq, *dk, *dv;
 };
 
 template <int D, bool CAP, bool DIST>
@@ -685,10 +694,10 @@ int launch_bwd(const BwdMaps& m, const MaskedBwdParams& p0, const MaskedBwdParam
   if (!limit0.raise(masked_bwd_kernel<D, 0, CAP, DIST>, smem0) || !limit1.raise(masked_bwd_kernel<D, 1, CAP, DIST>, smem1))
     return -10;
   gfs_host::launch_pdl(masked_bwd_kernel<D, 0, CAP, DIST>, dim3(items0), dim3(MBWD_THREADS), smem0, stream, *m.k128,
-                       *m.v128, *m.q64, *m.do64, p0, n_rt);
+                       *m.v128, *m.q64, *m.do64, *m.dk, *m.dv, p0, n_rt);
   if (cudaGetLastError() != cudaSuccess) return -12;
   gfs_host::launch_pdl(masked_bwd_kernel<D, 1, CAP, DIST>, dim3(items1), dim3(MBWD_THREADS), smem1, stream, *m.q128,
-                       *m.do128, *m.k64, *m.v64, p1, n_rt);
+                       *m.do128, *m.k64, *m.v64, *m.dq, *m.dq, p1, n_rt);
   return cudaGetLastError() == cudaSuccess ? 0 : -13;
 }
 template <int D>
@@ -747,8 +756,12 @@ int gfs_masked_attention_bwd(const void* q, const void* k, const void* v, const 
   const BwdMaps maps{make_map(q, D, S, nh, B, sq, 128), make_map(k, D, S, nkv, B, sk, 128),
                      make_map(v, D, S, nkv, B, sv, 128), make_map(dout, D, S, nh, B, sdo, 128),
                      make_map(q, D, S, nh, B, sq, 64), make_map(k, D, S, nkv, B, sk, 64),
-                     make_map(v, D, S, nkv, B, sv, 64), make_map(dout, D, S, nh, B, sdo, 64)};
-  if (!maps.q128 || !maps.k128 || !maps.v128 || !maps.do128 || !maps.q64 || !maps.k64 || !maps.v64 || !maps.do64) return -3;
+                     make_map(v, D, S, nkv, B, sv, 64), make_map(dout, D, S, nh, B, sdo, 64),
+                     make_map(dq, D, S, nh, B, sdq, 32, 32), make_map(dk, D, S, nkv, B, sdk, 32, 32),
+                     make_map(dv, D, S, nkv, B, sdv, 32, 32)};
+  if (!maps.q128 || !maps.k128 || !maps.v128 || !maps.do128 || !maps.q64 || !maps.k64 || !maps.v64 || !maps.do64 ||
+      !maps.dq || !maps.dk || !maps.dv)
+    return -3;
   p.lse = static_cast<const float*>(saved);
   p.dvec = static_cast<const float*>(dvec);
   p.S = S; p.S_pad = S_pad; p.B = B; p.nh = nh; p.group = nh / nkv; p.scale = scale;
@@ -757,14 +770,11 @@ int gfs_masked_attention_bwd(const void* q, const void* k, const void* v, const 
   p.score.slopes = static_cast<const float*>(slopes);
   p.status = gfs_host::status_words();
   p.parts = 1;
-  MaskedBwdParams p0 = p, p1 = p;
+  MaskedBwdParams p0 = p;
   p0.parts = group_parts(S_pad / 128, B, nkv, nh / nkv);
   p0.partial = static_cast<float*>(partial);
-  p0.out1 = static_cast<__nv_bfloat16*>(dk); p0.o1_ss = sdk[0]; p0.o1_bs = sdk[1]; p0.o1_hs = sdk[2];
-  p0.out2 = static_cast<__nv_bfloat16*>(dv); p0.o2_ss = sdv[0]; p0.o2_bs = sdv[1]; p0.o2_hs = sdv[2];
-  p1.out1 = static_cast<__nv_bfloat16*>(dq); p1.o1_ss = sdq[0]; p1.o1_bs = sdq[1]; p1.o1_hs = sdq[2];
-  const int rc = D == 64 ? launch_bwd_scores<64>(maps, p0, p1, cap > 0.f, stream)
-                         : launch_bwd_scores<128>(maps, p0, p1, cap > 0.f, stream);
+  const int rc = D == 64 ? launch_bwd_scores<64>(maps, p0, p, cap > 0.f, stream)
+                         : launch_bwd_scores<128>(maps, p0, p, cap > 0.f, stream);
   if (rc != 0 || p0.parts == 1) return rc;
   const long long rows = 2ll * B * nkv * S;
   const int rows_per_block = 256 / (D >> 3);
