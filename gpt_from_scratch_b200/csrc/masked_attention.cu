@@ -4,7 +4,6 @@
 //   out_i = sum_j p_ij v_j,  p_ij = 2^(score_ij - lse_i) over the keys j that query i sees; a query that sees none: 0
 //
 // One pass over the keys with the running maximum and sum of the softmax; heads of q share the heads of k and v in groups.
-#include <algorithm>
 
 #include "api.h"
 #include "attention_tiles.cuh"
