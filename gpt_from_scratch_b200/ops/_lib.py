@@ -13,6 +13,7 @@ from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_uint32, c_void
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 # GFS_LIB_PATH selects another build of the library (e.g. an experimental variant) explicitly.
 _LIB_PATH = Path(os.environ.get("GFS_LIB_PATH") or
@@ -201,12 +202,27 @@ def on_device(t: torch.Tensor):
     return _NULL_RANGE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
+def bare(*tensors: torch.Tensor | None) -> bool:
+    """An operator on these may call its kernel without its autograd function (10 us less): none asks for a gradient, and nobody
+    is making forward-mode derivatives or a trace, which see functions but no pointers. The function refuses tangents, and a
+    trace calls it again."""
+    if forward_ad._current_level >= 0 or torch._C._is_tracing():
+        return False
+    return not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
+
+
 def first_order(backward):
     """A ``Function.backward`` that autograd cannot differentiate again: ``once_differentiable`` where a graph of the
-    backward is being made, the bare function (8 us less) where none is."""
+    backward is being made, the bare function (8 us less) where none is. Gradients with tangents (forward mode over
+    reverse mode) and traces of a backward are refused: both would go on from results that only pointers have seen. (The
+    thread that runs the backward does not know of the trace: the function's forward sets ``ctx.traced``.)"""
     guarded = torch.autograd.function.once_differentiable(backward)
 
     def run(ctx, *grads):
+        if forward_ad._current_level >= 0 and any(g is not None and forward_ad.unpack_dual(g).tangent is not None for g in grads):
+            raise NotImplementedError("the backward of this operator has no forward-mode derivative")
+        if ctx.traced:
+            raise NotImplementedError("the backward of this operator cannot be traced")
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return run
 

@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import operator
 
 import torch
 
@@ -89,6 +90,24 @@ def _mask_reference(batch, seq_len, causal, ids, prefix, window, device):
     return AttentionMask(batch, S, device, parts=(first.int(), last.int(), (at - start).int()))
 
 
+def _mask_buffer(B, S, ids, prefix, causal, window, device) -> torch.Tensor:
+    buffer = torch.empty(_layout(B, S)["end"], dtype=torch.int32, device=device)
+    with _lib.on_device(buffer), _lib.nvtx("attention_mask"):
+        rc = _lib.lib().gfs_attention_mask(_lib.ptr(ids), ids is not None and ids.dtype == torch.int64, _lib.ptr(prefix), B,
+                                           S, causal, window, buffer.data_ptr(), _lib.stream_ptr())
+    _lib.check(rc, "gfs_attention_mask")
+    return buffer
+
+
+class _MaskBuffer(torch.autograd.Function):
+    """For traces, which see a function where they miss a pointer."""
+    @staticmethod
+    def forward(ctx, *args):
+        buffer = _mask_buffer(*args)
+        ctx.mark_non_differentiable(buffer)
+        return buffer
+
+
 def attention_mask(batch: int, seq_len: int, causal: bool = True, document_ids: torch.Tensor | None = None,
                    prefix_mask: torch.Tensor | None = None, window: int | None = None, device=None) -> AttentionMask:
     """The mask of ``batch`` sequences of ``seq_len`` tokens for :func:`masked_attention`.
@@ -99,6 +118,7 @@ def attention_mask(batch: int, seq_len: int, causal: bool = True, document_ids: 
     by all of it. ``window`` (causal only): a token sees no token more than ``window - 1`` before it. ``device`` defaults to
     the tensors' one, without tensors to the CPU. On CUDA one launch.
     """
+    batch, seq_len = operator.index(batch), operator.index(seq_len)      # (in traces, sizes are tensors)
     if batch < 0 or seq_len < 0:
         raise ValueError(f"attention_mask: {batch} sequences of {seq_len} tokens do not do")
     if document_ids is not None and (document_ids.shape != (batch, seq_len) or
@@ -120,13 +140,8 @@ def attention_mask(batch: int, seq_len: int, causal: bool = True, document_ids: 
         return _mask_reference(batch, seq_len, causal, document_ids, prefix_mask, window, device)
     ids = None if document_ids is None else document_ids.contiguous()
     prefix = None if prefix_mask is None else prefix_mask.contiguous()
-    B, S = batch, seq_len
-    buffer = torch.empty(_layout(B, S)["end"], dtype=torch.int32, device=device)
-    with _lib.on_device(buffer), _lib.nvtx("attention_mask"):
-        rc = _lib.lib().gfs_attention_mask(_lib.ptr(ids), ids is not None and ids.dtype == torch.int64, _lib.ptr(prefix), B,
-                                           S, causal, min(window or 0, 0x7fffffff), buffer.data_ptr(), _lib.stream_ptr())
-    _lib.check(rc, "gfs_attention_mask")
-    return AttentionMask(B, S, device, buffer)
+    make = _mask_buffer if _lib.bare(ids, prefix) else _MaskBuffer.apply
+    return AttentionMask(batch, seq_len, device, make(batch, seq_len, ids, prefix, causal, min(window or 0, 0x7fffffff), device))
 
 
 def masked_attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: AttentionMask, softcap: float = 0.0,
@@ -201,6 +216,7 @@ class _MaskedAttention(torch.autograd.Function):
         out, saved = _forward(q, k, v, buffer, slopes, softcap, scale, True)
         ctx.save_for_backward(q, k, v, out, saved, buffer, slopes)
         ctx.args = (softcap, scale)
+        ctx.traced = torch._C._is_tracing()
         return out
 
     @staticmethod
@@ -238,7 +254,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
     ``slope * |i - j|``. A query that sees nothing gets zeros, and what padding holds does not matter; a value that is not
     finite elsewhere may spread to queries of its 128-token tile that do not see it. The result is laid out like q. On CUDA:
     bfloat16, D 64 or 128 and softcap up to 1000, any strides (copied first where a dimension is broadcast or 16-byte accesses
-    do not reach), deterministic; other devices: torch operations.
+    do not reach), deterministic, no forward-mode derivatives; other devices: torch operations.
     """
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError(f"masked_attention: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not fit")
@@ -270,7 +286,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
         if B > 65535 or _pad128(S) * nh >= 2 ** 30 or _pad128(S) // 128 * B * nh >= 2 ** 31:
             raise ValueError(f"masked_attention: {B} sequences of {S} tokens with {nh} heads are too many for one call")
         slopes = None if alibi_slopes is None else alibi_slopes.contiguous()
-        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-            return _MaskedAttention.apply(q, k, v, mask.buffer, slopes, float(softcap), float(scale))
-        return _forward(_readable(q), _readable(k), _readable(v), mask.buffer, slopes, float(softcap), float(scale), False)[0]
+        if _lib.bare(q, k, v):
+            return _forward(_readable(q), _readable(k), _readable(v), mask.buffer, slopes, float(softcap), float(scale), False)[0]
+        return _MaskedAttention.apply(q, k, v, mask.buffer, slopes, float(softcap), float(scale))
     return masked_attention_reference(q, k, v, mask, softcap, alibi_slopes, scale)

@@ -49,6 +49,7 @@ class _QkNormRope(torch.autograd.Function):
     def forward(ctx, qkv, q_weight, k_weight, cos, sin, n1, n2, eps, positions, interleaved):
         ctx.save_for_backward(qkv, q_weight, k_weight, cos, sin, positions)
         ctx.args = (n1, n2, eps, interleaved)
+        ctx.traced = torch._C._is_tracing()
         return _forward(qkv, q_weight, k_weight, cos, sin, n1, n2, eps, positions, interleaved)
 
     @staticmethod
@@ -89,7 +90,7 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: tor
     q and k are normalised per head with ``q_weight``, ``k_weight [D]`` (of qkv's type; both ``None``: rotated only) and
     rotated as by :func:`~gpt_from_scratch_b200.ops.rope.rotary`, which documents ``cos``, ``sin``, ``positions`` and
     ``interleaved``; v is a view into ``qkv`` (not to be written to). Gradients for qkv and both weights. On CUDA:
-    bfloat16, float16 or float32 and D up to 256.
+    bfloat16, float16 or float32 and D up to 256, no forward-mode derivatives.
     """
     if num_heads < 0 or num_kv_heads < 0 or num_heads + num_kv_heads == 0:
         raise ValueError(f"qk_norm_rope: {num_heads} and {num_kv_heads} heads do not do")
@@ -111,8 +112,5 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: tor
             q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
         args = (rows_of(qkv), q_weight, k_weight, cos.contiguous(), sin.contiguous(), num_heads, num_kv_heads, float(eps),
                 None if positions is None else positions.contiguous(), bool(interleaved))
-        if torch.is_grad_enabled() and (qkv.requires_grad or (q_weight is not None and
-                                                              (q_weight.requires_grad or k_weight.requires_grad))):
-            return _QkNormRope.apply(*args)
-        return _forward(*args)
+        return _forward(*args) if _lib.bare(qkv, q_weight, k_weight) else _QkNormRope.apply(*args)
     return qk_norm_rope_reference(qkv, q_weight, k_weight, cos, sin, num_heads, num_kv_heads, eps, positions, interleaved)

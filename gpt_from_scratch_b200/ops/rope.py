@@ -208,6 +208,7 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, x, cos, sin, positions, interleaved):
         ctx.save_for_backward(cos, sin, positions)
         ctx.interleaved = interleaved
+        ctx.traced = torch._C._is_tracing()
         return _rotary_native(x, cos, sin, positions, interleaved, False)
 
     @staticmethod
@@ -225,7 +226,8 @@ def rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: tor
     row ``s``, or ``positions[b, s]`` (int32 or int64 ``[B, S]``): documents packed into a sequence, tokens far
     into a context. ``interleaved``: pairs ``(2i, 2i + 1)`` as in :func:`apply_rope`, else ``(i, i + R / 2)``. ``x`` may have
     any strides; the result is a new contiguous tensor of its type. On CUDA: bfloat16, float16 or float32 and D up to
-    256; a position outside of the tables is reported by ``_lib.raise_on_status()`` (on the CPU: ValueError).
+    256, no forward-mode derivatives; a position outside of the tables is reported by ``_lib.raise_on_status()`` (on the CPU:
+    ValueError).
     """
     if x.dim() != 4:
         raise ValueError(f"rotary: x of shape {tuple(x.shape)} is not [S, B, heads, D]")
@@ -233,7 +235,5 @@ def rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: tor
     check_tables("rotary", x, cos, sin, positions, S, B, D)
     if x.is_cuda:
         args = (x, cos.contiguous(), sin.contiguous(), None if positions is None else positions.contiguous(), interleaved)
-        if torch.is_grad_enabled() and x.requires_grad:
-            return _Rotary.apply(*args)
-        return _rotary_native(*args, False)
+        return _rotary_native(*args, False) if _lib.bare(x) else _Rotary.apply(*args)
     return rotary_reference(x, cos, sin, positions, interleaved)
