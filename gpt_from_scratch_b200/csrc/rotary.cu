@@ -343,7 +343,9 @@ qk_norm_rope_bwd_kernel(const RotaryArgs a, unsigned n_items, unsigned items_per
           ss = fma_f32x2(v[e], v[e], ss);
           dot = fma_f32x2(zw[e], v[e], dot);
         }
-        const float rstd = rsqrtf(group_sum<LANES>(pair_sum(ss)) * a.inv_D + a.eps);
+        // (groups past the last head hold zeros, whose factor without eps would be infinite)
+        const float mean = group_sum<LANES>(pair_sum(ss)) * a.inv_D + a.eps;
+        const float rstd = on ? rsqrtf(mean) : 0.f;
         const float m = group_sum<LANES>(pair_sum(dot)) * rstd * rstd * a.inv_D;      // mean(dz w n) rstd
         const uint64_t r2 = pack_f32x2(rstd, rstd), m2 = pack_f32x2(-m, -m);
 #pragma unroll
