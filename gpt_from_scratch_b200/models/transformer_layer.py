@@ -10,7 +10,7 @@ the reference's CLI can reach) the residual adds run inside the row-parallel GEM
 With norms of q and k, capped scores, a window or documents (``config.qk_norm`` and the fields next to it) the packed
 projection goes through :func:`~gpt_from_scratch_b200.ops.qk_norm_rope.qk_norm_rope` and
 :func:`~gpt_from_scratch_b200.ops.masked_attention.masked_attention` instead, under a mask that the model makes once for
-all blocks.
+all blocks; a block that is called without one makes its own, except for documents, which it cannot know.
 """
 from __future__ import annotations
 
@@ -19,7 +19,7 @@ import torch.nn as nn
 
 from ..ops.attention import attention_reference, fused_rope_attention
 from ..ops.dropout import dropout_add
-from ..ops.masked_attention import AttentionMask, masked_attention, masked_attention_reference
+from ..ops.masked_attention import AttentionMask, attention_mask, masked_attention, masked_attention_reference
 from ..ops.qk_norm_rope import qk_norm_rope, qk_norm_rope_reference
 from ..ops.rope import rope_reference
 from ..parallel import parallel_state as ps
@@ -57,16 +57,22 @@ class ParallelAttention(nn.Module):
         self.attention_impl = getattr(config, "attention_impl", "fused")
         self.softcap = getattr(config, "attention_softcap", 0.0)
         self.masked = needs_mask(config)
+        self.window = getattr(config, "attention_window", 0)
+        self.documents = getattr(config, "eod_token_id", -1) >= 0
         if getattr(config, "qk_norm", False):
             self.q_norm = RMSNorm(self.head_dim, config.rms_norm_eps)
             self.k_norm = RMSNorm(self.head_dim, config.rms_norm_eps)
         else:
             self.q_norm = self.k_norm = None
 
-    def _masked(self, hidden_states, residual, mask: AttentionMask):
+    def _masked(self, hidden_states, residual, mask: AttentionMask | None):
         nh, D = self.num_heads_per_partition, self.head_dim
+        if mask is None and self.documents:
+            raise ValueError("attention over documents (eod_token_id) needs the mask that the model makes of its tokens")
         qkv = self.qkv_proj(hidden_states)                 # [S, B, 3H/P]
         S, B, _ = qkv.shape
+        if mask is None:
+            mask = attention_mask(B, S, window=self.window or None, device=qkv.device)
         cos, sin = self.rotary_emb(qkv, S)
         if cos.dtype in (torch.bfloat16, torch.float16):   # a model that was cast as a whole
             cos, sin = cos.float(), sin.float()
@@ -81,7 +87,7 @@ class ParallelAttention(nn.Module):
         return self.out_proj(ctx.permute(2, 0, 1, 3).reshape(S, B, nh * D), residual)
 
     def forward(self, hidden_states, residual=None, mask: AttentionMask | None = None):
-        if mask is not None:
+        if mask is not None or self.masked:
             return self._masked(hidden_states, residual, mask)
         nh, D = self.num_heads_per_partition, self.head_dim
         world = ps.get_tensor_model_parallel_world_size()
