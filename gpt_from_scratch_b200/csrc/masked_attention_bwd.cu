@@ -719,14 +719,13 @@ long long gfs_masked_attention_scratch(int S, int B, int nh, int nkv, int D) {
 }
 
 // strides: 24 element strides for {q, k, v, out, dout, dq, dk, dv} x {seq, batch, head}; lse (from the forward) and dvec
-// (scratch): fp32 [B, nh, S_pad]; partial: scratch of the
-// size above; the rest as for gfs_masked_attention_fwd. dq shares no memory with anything that is read
+// (scratch): fp32 [B, nh, S_pad]; partial: partial_floats of scratch, the size above on the same device or more (fewer are
+// refused: the parts depend on its SMs); the rest as for gfs_masked_attention_fwd. dq shares no memory with anything that is read
 // for dk and dv, nor with them: its kernel runs beside theirs.
 int gfs_masked_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout,
-                             const void* saved, void* dvec, void* partial, void* dq, void* dk, void* dv,
-                             const void* mask, int S, int B,
-                             int nh, int nkv, int D, const long long* strides, float scale, float cap, const void* slopes,
-                             void* stream_) {
+                             const void* saved, void* dvec, void* partial, long long partial_floats, void* dq, void* dk,
+                             void* dv, const void* mask, int S, int B, int nh, int nkv, int D, const long long* strides,
+                             float scale, float cap, const void* slopes, void* stream_) {
   if ((D != 64 && D != 128) || !strides_ok(strides, 24) || nkv <= 0 || nh % nkv != 0) return -1;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
        reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(dq) |
@@ -736,6 +735,8 @@ int gfs_masked_attention_bwd(const void* q, const void* k, const void* v, const 
   const int S_pad = (S + 127) / 128 * 128;
   if (static_cast<long long>(S_pad) * nh > 0x3fffffffll || B > 65535) return -1;   // 32-bit row numbers in the pre-pass
   if (static_cast<long long>(S_pad / 128) * B * nh > 0x7fffffffll) return -1;
+  const long long scratch = gfs_masked_attention_scratch(S, B, nh, nkv, D);
+  if (scratch > 0 && (partial == nullptr || reinterpret_cast<uintptr_t>(partial) & 15 || partial_floats < scratch)) return -4;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const long long *sq = strides, *sk = strides + 3, *sv = strides + 6, *so = strides + 9, *sdo = strides + 12,
                   *sdq = strides + 15, *sdk = strides + 18, *sdv = strides + 21;

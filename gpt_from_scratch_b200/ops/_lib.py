@@ -70,7 +70,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "gfs_masked_attention_fwd": ([vp, vp, vp, vp, vp, vp, i, i, i, i, i, lp, f, f, vp, vp], i),
         "gfs_attention_mask_layout": ([i, i, lp], None),
         "gfs_masked_attention_scratch": ([i, i, i, i, i], i64),
-        "gfs_masked_attention_bwd": ([vp] * 12 + [i, i, i, i, i, lp, f, f, vp, vp], i),
+        "gfs_masked_attention_bwd": ([vp] * 8 + [i64] + [vp] * 4 + [i, i, i, i, i, lp, f, f, vp, vp], i),
         "gfs_rotary": ([vp, vp, lp, vp, vp, vp, i, i, i, i, i, i, i, i, i, i, vp], i),
         "gfs_qk_norm_rope_fwd": ([vp, lp, vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, i, i, f, i, vp], i),
         "gfs_qk_norm_rope_scratch": ([i], i64),

@@ -205,7 +205,8 @@ def _forward(q, k, v, buffer, slopes, softcap: float, scale: float, training: bo
 
 
 @functools.lru_cache(maxsize=256)
-def _scratch(S: int, B: int, nh: int, nkv: int, D: int) -> int:
+def _scratch(S: int, B: int, nh: int, nkv: int, D: int, device: int = 0) -> int:
+    """fp32 elements that the backward wants on ``device``, the current one (it depends on the number of its SMs)."""
     return _lib.lib().gfs_masked_attention_scratch(S, B, nh, nkv, D)
 
 
@@ -231,14 +232,14 @@ class _MaskedAttention(torch.autograd.Function):
         kv = k.shape
         dout = _readable(dout)
         dvec = torch.empty(B * nh * _pad128(S), dtype=torch.float32, device=q.device)
-        scratch = _scratch(S, B, nh, kv[1], D)
-        partial = torch.empty(scratch, dtype=torch.float32, device=q.device) if scratch else None
         st = _stride_array(shape, q.stride(), kv, k.stride(), kv, v.stride(), shape, out.stride(), shape, dout.stride(), shape,
                            dq.stride(), kv, dk.stride(), kv, dv.stride())
         with _lib.on_device(q), _lib.nvtx("masked_attention_bwd"):
+            scratch = _scratch(S, B, nh, kv[1], D, q.get_device())
+            partial = torch.empty(scratch, dtype=torch.float32, device=q.device) if scratch else None
             rc = _lib.lib().gfs_masked_attention_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                                                      dout.data_ptr(), saved.data_ptr(), dvec.data_ptr(), _lib.ptr(partial),
-                                                     dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), buffer.data_ptr(), S, B,
+                                                     scratch, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), buffer.data_ptr(), S, B,
                                                      nh, kv[1], D, st, scale, softcap, _lib.ptr(slopes), _lib.stream_ptr())
         _lib.check(rc, "gfs_masked_attention_bwd")
         _lib.add_launches(3 if scratch else 2)  # pre-pass + two main kernels (+ the sum of the parts)
