@@ -346,9 +346,10 @@ struct MFwdShape {
 };
 // Scores: as they are, capped with a bound that the running maximum may be left out for, capped.
 enum Scores { PLAIN = 0, BOUNDED = 1, CAPPED = 2 };
-// Up to this cap2 no maximum is needed: probabilities lie within 2^-80 and 2^80, which leaves fp32 sums (and bf16, which has the
-// same exponents) a factor of 2^46 on either side.
-constexpr float BOUNDED_CAP2 = 80.f;
+// Up to this cap2 (caps up to 50) no maximum is needed: probabilities lie within 2^-73 and 2^73. What fp32 has beyond that is left to
+// the values: sums over 2^20 keys stay below 2^128 for magnitudes up to 2^30, products above 2^-126 for those from 2^-40 on, and that is
+// the range that masked_attention documents. With the maximum, us: 64 heads of 4096 under a window, cap 50, 221 -> 248.
+constexpr float BOUNDED_CAP2 = 73.f;
 
 template <int D, int SCORES, bool DIST>
 __global__ void __launch_bounds__(MFWD_THREADS, 1)

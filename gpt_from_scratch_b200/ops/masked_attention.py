@@ -254,7 +254,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
     ``softcap`` c > 0 ``c tanh(scale * q k / c)``, with ``alibi_slopes`` (fp32 ``[heads]``, constants for autograd) minus
     ``slope * |i - j|``. A query that sees nothing gets zeros, and what padding holds does not matter; a value that is not
     finite elsewhere may spread to queries of its 128-token tile that do not see it. The result is laid out like q. On CUDA:
-    bfloat16, D 64 or 128 and softcap up to 1000, any strides (copied first where a dimension is broadcast or 16-byte accesses
+    bfloat16, D 64 or 128 and softcap up to 1000 (up to 50: with magnitudes of v, where not 0, from 2^-40, below which digits are lost
+    where all scores are near the negative cap, to 2^30, above which sums may overflow where they are near the cap), any strides (copied first where a dimension is broadcast or 16-byte accesses
     do not reach), deterministic, no forward-mode derivatives; other devices: torch operations.
     """
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
