@@ -276,10 +276,9 @@ __global__ void __launch_bounds__(MASK_THREADS) attention_mask_kernel(const Mask
     const int la = first[t * 256], ha = end(last, 2 * t);
     const int lb = two ? first[t * 256 + 128] : 0, hb = two ? end(last, 2 * t + 1) : 0;
     int a0 = la >> 6, a1 = (ha + 63) >> 6, b0 = lb >> 6, b1 = (hb + 63) >> 6;
-    if (a1 <= a0) {               // all padding: one block, of the other tile's
-      a0 = two && b1 > b0 ? b0 : a0;
-      a1 = a0 + 1;
-    }
+    // A row's range holds its own place or, of padding, ends there: only a tile of one row that is padding may have no block, the
+    // last of a sequence. It gets one, which is masked whole; behind another tile that one's last, so that no gap comes between them.
+    if (a1 <= a0) a1 = a0 + 1;
     if (two && b1 <= b0) {
       b0 = a1 - 1;
       b1 = a1;
