@@ -24,13 +24,13 @@ class GPTConfig:
     init_method: str = "xavier_uniform"   # or "normal"
     init_std: float = 0.02
     attention_impl: str = "fused"         # "fused": tcgen05 flash attention on CUDA; "torch": eager oracle
+    reference_quirks: bool = False        # reproduce reference behaviours that were fixed by default
     rope_scaling: RopeScaling | None = None  # angles for contexts longer than trained on (ops/rope.py)
     # Any of these four sends attention through ops/qk_norm_rope.py and ops/masked_attention.py:
     qk_norm: bool = False                 # RMSNorm of every head of q and k, before the rotation
     attention_softcap: float = 0.0        # c > 0: scores become c tanh(score / c)
     attention_window: int = 0             # w > 0: no token sees one more than w - 1 before it
     eod_token_id: int = -1                # >= 0: documents end with it, tokens see (and count positions in) their own only
-    reference_quirks: bool = False        # reproduce reference behaviours that were fixed by default
 
     def flops_per_token(self, seq_len: int) -> float:
         """Forward+backward matmul FLOPs per token (causal attention counted at half)."""
