@@ -60,7 +60,7 @@ def parse_args(argv=None):
                    help="id >= 0 that ends a document: tokens see only their own document")
     p.add_argument("--rope-scaling", choices=["linear", "ntk", "by_parts"], default=None,
                    help="rotary angles for contexts longer than trained on (ops/rope.py: RopeScaling)")
-    p.add_argument("--rope-scaling-factor", type=float, default=1.0)
+    p.add_argument("--rope-scaling-factor", type=float, default=None, help="needed by --rope-scaling: times the context grows")
     p.add_argument("--rope-original-length", type=int, default=0, help="context that by_parts scaling starts from")
     p.add_argument("--comm-impl", choices=["fused", "nccl"], default="nccl",
                    help="fused: peer-memory kernels that overlap the collective with the GEMM")
@@ -80,7 +80,12 @@ def parse_args(argv=None):
     p.add_argument("--heartbeat-timeout", type=float, default=300.0,
                    help="seconds a peer may lag behind at a log interval before PeerFailure is raised "
                         "(0 disables the heartbeat)")
-    return p.parse_args(argv)
+    args = p.parse_args(argv)
+    if (args.rope_scaling is None) != (args.rope_scaling_factor is None):
+        p.error("--rope-scaling and --rope-scaling-factor go together")
+    if args.rope_original_length and args.rope_scaling != "by_parts":
+        p.error("--rope-original-length goes with --rope-scaling by_parts")
+    return args
 
 
 def build_config(args) -> GPTConfig:
