@@ -32,10 +32,18 @@ class GPTConfig:
     attention_window: int = 0             # w > 0: no token sees one more than w - 1 before it
     eod_token_id: int = -1                # >= 0: documents end with it, tokens see (and count positions in) their own only
 
-    def flops_per_token(self, seq_len: int) -> float:
-        """Forward+backward matmul FLOPs per token (causal attention counted at half)."""
+    def keys_per_token(self, seq_len: int) -> float:
+        """Keys that a token of a whole sequence sees on average, the causal half of it (itself counted at half) or what the window
+        leaves of that. Documents see less, by their lengths."""
+        w = min(self.attention_window or seq_len, seq_len)
+        return w - w * w / (2.0 * seq_len) if seq_len else 0.0
+
+    def flops_per_token(self, seq_len: int, keys: float | None = None) -> float:
+        """Forward+backward matmul FLOPs per token, of attention those for the ``keys`` that a token sees on average
+        (:meth:`keys_per_token`)."""
         H, I, L, V = self.hidden_size, self.intermediate_size, self.num_layers, self.vocab_size
-        return 3.0 * (L * (2.0 * (4 * H * H + 3 * H * I) + 2.0 * seq_len * H) + 2.0 * H * V)
+        keys = self.keys_per_token(seq_len) if keys is None else keys
+        return 3.0 * (L * (2.0 * (4 * H * H + 3 * H * I) + 4.0 * keys * H) + 2.0 * H * V)
 
     def num_parameters(self) -> int:
         H, I, L, V = self.hidden_size, self.intermediate_size, self.num_layers, self.vocab_size

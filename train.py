@@ -102,6 +102,12 @@ def build_config(args) -> GPTConfig:
         eod_token_id=args.eod_token_id)
 
 
+def keys_of_documents(config: GPTConfig, mask) -> torch.Tensor:
+    """GPTConfig.keys_per_token of a batch of documents, from its mask."""
+    keys = mask.positions.float() + 0.5
+    return keys.clamp_max(config.attention_window or float("inf")).mean()
+
+
 def init_distributed(args):
     use_cuda = (args.device or ("cuda" if torch.cuda.is_available() else "cpu")) == "cuda"
     if "RANK" in os.environ and "WORLD_SIZE" in os.environ:
@@ -166,7 +172,9 @@ def main(argv=None):
     batches = PrefetchLoader(loader, device) if use_cuda else loader
     log_loss = torch.zeros((), dtype=torch.float32, device=device)
     log_start = time.time()
-    flops_per_token = config.flops_per_token(args.seq_len)
+    # for the utilisation; the keys that tokens of documents see are summed up over a log interval (rank 0's: it writes the log)
+    count_keys = bool(args.peak_tflops) and config.eod_token_id >= 0 and rank == 0
+    keys = torch.zeros((), dtype=torch.float32, device=device)
     while step < args.max_steps:
         sampler.set_epoch(epoch)
         if batches_in_epoch:
@@ -183,6 +191,8 @@ def main(argv=None):
             step += 1
             batches_in_epoch += 1
             log_loss += loss.float()
+            if count_keys:
+                keys += keys_of_documents(config, engine.model.attention_mask(inputs))
             if heartbeat is not None:
                 heartbeat.beat(step)
             if step % args.log_interval == 0:
@@ -198,7 +208,9 @@ def main(argv=None):
                 if engine.optimizer.last_grad_norm is not None:
                     rec["grad_norm"] = float(engine.optimizer.last_grad_norm)
                 if args.peak_tflops:
-                    rec["mfu"] = tps * flops_per_token / (world * args.peak_tflops * 1e12)
+                    seen = float(keys) / args.log_interval if count_keys else None
+                    rec["mfu"] = tps * config.flops_per_token(args.seq_len, seen) / (world * args.peak_tflops * 1e12)
+                    keys.zero_()
                 if use_cuda:
                     rec["peak_mem_gb"] = torch.cuda.max_memory_allocated() / 2 ** 30
                     from gpt_from_scratch_b200.ops import _lib
