@@ -119,7 +119,7 @@ def attention_mask(batch: int, seq_len: int, causal: bool = True, document_ids: 
     the tensors' one, without tensors to the CPU. On CUDA one launch.
     """
     batch, seq_len = operator.index(batch), operator.index(seq_len)      # (in traces, sizes are tensors)
-    if batch < 0 or seq_len < 0:
+    if not (0 <= batch < 2 ** 31 and 0 <= seq_len <= 0x3fff0000):       # 32-bit places, also behind a window
         raise ValueError(f"attention_mask: {batch} sequences of {seq_len} tokens do not do")
     if document_ids is not None and (document_ids.shape != (batch, seq_len) or
                                      document_ids.dtype not in (torch.int32, torch.int64)):
@@ -271,8 +271,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
     if not (softcap >= 0.0 and math.isfinite(softcap)):
         raise ValueError(f"masked_attention: softcap {softcap} is neither 0 nor positive")
     scale = 1.0 / math.sqrt(D) if scale is None and D else scale
-    if scale is not None and not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError(f"masked_attention: scale {scale} is not positive")
+    if scale is not None and not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"masked_attention: scale {scale} is not positive, or so far from 1 that 32 bits cannot hold it with a cap")
     if alibi_slopes is not None:
         if alibi_slopes.shape != (nh,) or alibi_slopes.dtype != torch.float32 or alibi_slopes.device != q.device:
             raise ValueError(f"masked_attention: alibi_slopes have to be fp32 of shape [{nh}] on {q.device}")
