@@ -874,7 +874,7 @@ int gfs_attention_mask(const void* ids, int ids64, const void* prefix, int B, in
                        void* stream) {
   if (S < 0 || B < 0 || window < 0 || (!causal && (window > 0 || prefix != nullptr)) || S > 0x3fff0000) return -1;   // (i + window fits an int)
   if (S == 0 || B == 0) return 0;
-  if (reinterpret_cast<uintptr_t>(out) & 15) return -2;
+  if (out == nullptr || reinterpret_cast<uintptr_t>(out) & 15) return -2;
   int* o = static_cast<int*>(out);
   const MaskLayout l = mask_layout(B, S);
   const MaskArgs a{ids, static_cast<const uint8_t*>(prefix), ids64, S, (S + 127) / 128 * 128, window > S ? 0 : window, causal,
@@ -906,6 +906,7 @@ int gfs_masked_attention_fwd(const void* q, const void* k, const void* v, void* 
        reinterpret_cast<uintptr_t>(out)) & 15 || reinterpret_cast<uintptr_t>(saved) & 31)
     return -2;
   if (S <= 0 || B <= 0 || nh <= 0) return 0;
+  if (mask == nullptr) return -2;
   const int S_pad = (S + 127) / 128 * 128;
   if (static_cast<long long>(S_pad / 128) * B * nh > 0x7fffffffll) return -1;
   const FwdMaps m{make_map(q, D, S, nh, B, strides + 0, 128), make_map(k, D, S, nkv, B, strides + 3, 64),

@@ -713,6 +713,7 @@ extern "C" {
 
 // fp32 elements of the scratch `partial` of the backward (0: none)
 long long gfs_masked_attention_scratch(int S, int B, int nh, int nkv, int D) {
+  if (S <= 0 || B <= 0 || nh <= 0 || nkv <= 0) return 0;
   const int tiles = (S + 127) / 128;
   const int parts = group_parts(tiles, B, nkv, nh / nkv);
   return parts > 1 ? 2ll * parts * B * nkv * tiles * 128 * D : 0;
@@ -735,6 +736,7 @@ int gfs_masked_attention_bwd(const void* q, const void* k, const void* v, const 
   const int S_pad = (S + 127) / 128 * 128;
   if (static_cast<long long>(S_pad) * nh > 0x3fffffffll || B > 65535) return -1;   // 32-bit row numbers in the pre-pass
   if (static_cast<long long>(S_pad / 128) * B * nh > 0x7fffffffll) return -1;
+  if (saved == nullptr || dvec == nullptr || mask == nullptr) return -2;
   const long long scratch = gfs_masked_attention_scratch(S, B, nh, nkv, D);
   if (scratch > 0 && (partial == nullptr || reinterpret_cast<uintptr_t>(partial) & 15 || partial_floats < scratch)) return -4;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);

@@ -688,6 +688,7 @@ int gfs_qk_norm_rope_bwd(const void* x, const void* dq, const void* dk, const vo
                          int R, int half, float eps, int dtype, void* stream) {
   if (!sizes_ok(S, B, n1 + n2, D, R, rows, positions)) return -1;
   if ((w1 == nullptr) != (w2 == nullptr) || S == 0 || B == 0 || n1 + n2 == 0) return -1;
+  if (w1 != nullptr && (dw1 == nullptr || dw2 == nullptr || dw == nullptr)) return -1;
   RotaryArgs a = {};
   a.x = part(x, strides);
   a.y1 = part(dq, strides + 3);

@@ -49,3 +49,20 @@ def test_every_device_of_a_process_is_served(fake, D, cap, slopes):  # noqa: F81
         assert fake.gfs_masked_attention_fwd(*[BUF] * 6, 300, 1, 8, 8, D, strides, 0.1, cap, slopes, 0) == 0
         assert fake.gfs_masked_attention_bwd(*[BUF] * 8, 1 << 30, *[BUF] * 4, 300, 1, 8, 8, D, strides, 0.1, cap, slopes, 0) == 0
     fake.fake_set_device(0)
+
+
+def test_entries_refuse_what_would_end_the_process(fake):  # noqa: F811
+    """No key heads (a division), no place for what a kernel writes."""
+    for sizes in ((300, 1, 8, 0, 64), (300, 1, 0, 0, 64), (0, 1, 8, 1, 64), (-5, 1, 8, 1, 64)):
+        assert fake.gfs_masked_attention_scratch(*sizes) == 0
+    before = fake.fake_launches()
+    strides = (ctypes.c_longlong * 24)(*[64, 64 * 300 * 8, 64 * 300] * 8)
+    for hole in (5, 6, 11):             # saved, dvec, mask
+        at = [0 if i == hole else BUF for i in range(12)]
+        assert fake.gfs_masked_attention_bwd(*at[:8], 1 << 30, *at[8:], 300, 1, 8, 8, 64, strides, 0.1, 0.0, 0, 0) != 0
+    assert fake.gfs_masked_attention_fwd(*[BUF] * 5, 0, 300, 1, 8, 8, 64, strides, 0.1, 0.0, 0, 0) != 0
+    assert fake.gfs_attention_mask(0, 0, 0, 1, 300, 1, 0, 0, 0) != 0
+    for hole in range(3):               # the weights' gradients and their scratch
+        dw = [0 if i == hole else BUF for i in range(3)]
+        assert fake.gfs_qk_norm_rope_bwd(*[BUF] * 5, strides, BUF, BUF, *dw, BUF, BUF, 0, 0, 300, 300, 1, 4, 2, 64, 64, 0, 1e-5, 0, 0) != 0
+    assert fake.fake_launches() == before
