@@ -26,7 +26,8 @@ class GPTConfig:
     attention_impl: str = "fused"         # "fused": tcgen05 flash attention on CUDA; "torch": eager oracle
     reference_quirks: bool = False        # reproduce reference behaviours that were fixed by default
     rope_scaling: RopeScaling | None = None  # angles for contexts longer than trained on (ops/rope.py)
-    # Any of these four sends attention through ops/qk_norm_rope.py and ops/masked_attention.py:
+    # Any of these four sends attention through ops/qk_norm_rope.py and ops/masked_attention.py (on CUDA their kernels in bf16 with
+    # heads of 64 or 128, else their torch forms, as without the four; attention then makes its S x S matrix):
     qk_norm: bool = False                 # RMSNorm of every head of q and k, before the rotation
     attention_softcap: float = 0.0        # c > 0: scores become c tanh(score / c)
     attention_window: int = 0             # w > 0: no token sees one more than w - 1 before it

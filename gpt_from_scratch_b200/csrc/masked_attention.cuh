@@ -83,7 +83,7 @@ __device__ __forceinline__ void sigmoids(uint64_t x0, uint64_t x1, uint64_t sl2,
 
 // What the rounding of outputs to bf16 leaves out, for the backward: dvec = sum dO O takes the place of sum P dP there, and in rows
 // that see a few keys, whose P (dP - dvec) is small against both, half a step of O (up to 2^-8) is more than all else that is rounded:
-// errors of dQ and dK are 2.7 to 3.2e-3 with it and 2.4 to 2.5e-3 without, in documents of 4 to 100 tokens up to 5.5e-3 and 2.5 to 3.1e-3.
+// errors of dQ and dK are 2.7 to 3.2e-3 with it and 2.4 to 2.5e-3 without, in documents of 4 to 100 tokens up to 5.5e-3 and 2.5 to 3.4e-3.
 // A signed byte per number, the next eight bits of its pattern as the difference from the rounded one (patterns grow with magnitudes, so
 // exponents and signs do not matter); it leaves 2^-15. Costs: half of O written and read once more, 4 to 5 % of a training call.
 __device__ __forceinline__ uint32_t bf16_rest(const float (&o)[4], uint32_t r01, uint32_t r23) {

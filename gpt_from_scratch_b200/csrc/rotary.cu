@@ -19,8 +19,10 @@
 // A row (the head of a token) belongs to a group of 8, 16 or 32 lanes, eight elements each (one 16-byte load of a 16-bit type); a
 // partner half a head away is in another lane of the group, and the norm's sums stay in it. A group takes a few rows
 // of one token, so that the table's entries are loaded once for them and the loads of all rows are in flight together.
-// What no 16-byte access can reach (odd sizes, strides or addresses) goes to kernels that give a row a warp, an
-// element at a time.
+// What no 16-byte access can reach (odd strides or addresses, head sizes no multiple of 8), and rotated dimensions whose halves or
+// pairs would part a lane's eight elements (no multiple of 16, or of 8 in pairs), go to kernels that give a row a warp, an
+// element at a time: right for everything, and far from memory's rate. us (beside them the 16-byte path's): 16 heads of 8192 tokens,
+// bf16, 40 of 80 halves apart 41 (all 80: 16), 24 of 96 47 (18); with norms and k's heads 100 (31), with the backward 496 (88).
 #include <cuda_fp16.h>
 
 #include <algorithm>

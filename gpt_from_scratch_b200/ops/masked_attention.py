@@ -252,11 +252,15 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
 
     Heads of q share those of k and v in groups of ``heads / kv_heads``. Scores are ``scale * q k`` (default ``1 / sqrt(D)``), with
     ``softcap`` c > 0 ``c tanh(scale * q k / c)``, with ``alibi_slopes`` (fp32 ``[heads]``, constants for autograd) minus
-    ``slope * |i - j|``. A query that sees nothing gets zeros, and what padding holds does not matter; a value that is not
-    finite elsewhere may spread to queries of its 128-token tile that do not see it. The result is laid out like q. On CUDA:
-    bfloat16, D 64 or 128 and softcap up to 1000 (up to 50: with magnitudes of v, where not 0, from 2^-40, below which digits are lost
-    where all scores are near the negative cap, to 2^30, above which sums may overflow where they are near the cap), any strides (copied first where a dimension is broadcast or 16-byte accesses
-    do not reach), deterministic, no forward-mode derivatives; other devices: torch operations.
+    ``slope * |i - j|``. A query that sees nothing gets zeros, and what padding holds does not matter. The result is laid out
+    like q. On CUDA: bfloat16, D 64 or 128 and softcap up to 1000, any strides (copied first where a dimension is broadcast or
+    16-byte accesses do not reach), deterministic, no forward-mode derivatives; other devices: torch operations.
+
+    On CUDA probabilities and the gradients of scores are rounded to bfloat16 before their products. With a softcap of up to 50
+    magnitudes of v, where not 0, have to lie between 2^-40, below which digits are lost where all of a query's scores are near the
+    negative cap, and 2^30, above which sums may overflow where they are near the cap. A value that is not finite, outside of padding,
+    may spread past the mask: a key's to all queries of a tile of 128 of which one sees any of the 64 keys of its block, and a
+    query's to the gradients of such keys.
     """
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError(f"masked_attention: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not fit")
