@@ -203,7 +203,7 @@ def on_device(t: torch.Tensor):
 
 
 def bare(*tensors: torch.Tensor | None) -> bool:
-    """An operator on these may call its kernel without its autograd function (10 us less): none asks for a gradient, and nobody
+    """An operator on these may call its kernel without its autograd function, which costs host time: none asks for a gradient, and nobody
     is making forward-mode derivatives or a trace, which see functions but no pointers. The function refuses tangents, and a
     trace calls it again."""
     if forward_ad._current_level >= 0 or torch._C._is_tracing():
